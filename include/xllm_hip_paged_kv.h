@@ -519,6 +519,183 @@ int xllm_hip_gather_from_cache(const xllm_hip_kv_cache* cache,
                                int32_t quant_mode,
                                xllm_hip_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * A speculative step over a tree of drafted tokens.  A draft model proposes, for every sequence, a tree
+ * whose nodes are the sequence's query tokens of the step; their K and V go into the cache behind the
+ * sequence's tokens, in the order of the nodes; the target model attends all of them in one call, each
+ * node seeing the context and its own ancestors; the tokens of one path are accepted and their cache
+ * rows move to the front.  In the order of a step:
+ *   xllm_hip_build_step_indices    lengths -> block tables, slot map, positions, list forms
+ *   xllm_hip_tree_masks            parents -> ancestor masks and positions
+ *   xllm_hip_mrope_kv_write        norm + rotary embedding (one or several position axes) + KV write
+ *   xllm_hip_tree_attention        attention under the masks
+ *   xllm_hip_move_accepted_tokens  accepted rows to the front, new lengths
+ * None of them reads anything back to the host, so a step whose lengths live on the device needs no
+ * synchronisation.  They have no counterpart in the reference, which drafts chains
+ * (xllm/core/runtime/speculative_worker_impl.cpp:230-243) and builds these arrays on the host
+ * (xllm/core/framework/batch/batch_input_builder.cpp:438-560).
+ * ------------------------------------------------------------------------------------------------ */
+
+/*
+ * Index arrays of a step from the requests' lengths, on the device.  With c = cached_lens[b] (tokens
+ * already in the cache), n = new_lens[b] (or q_per_seq), need = ceil((c + n) / block_size), r the
+ * sequence's row of block_pool, W = min(pool_width, table_width):
+ *   seq_lens[b] = c + n            q_indptr = exclusive sums of n, [batch + 1]
+ *   block i < need of the sequence:  block_pool[r][i]                                   for i < held
+ *                                    free_blocks[*free_head + sum of the sequences before + i - held]   above
+ *   block_table[b][i] = that block, 0 for i >= need, up to table_width
+ *   for j < n, row t = q_indptr[b] + j < num_rows:  positions[t] = c + j,
+ *                                    slot_mapping[t] = block((c + j) / block_size) * block_size + (c + j) % block_size
+ *   rows t from q_indptr[batch] to num_rows - 1 (the padding of a captured graph): slot -1, which every KV
+ *                                    write skips, and position 0
+ *   kv_indptr / kv_indices / kv_last_page_len: the same block lists in the CSR form (optional, together;
+ *                                    kv_indptr = exclusive sums of min(need, table_width); an empty sequence has
+ *                                    page length 0, one cut to table_width blocks a full last page; entries past
+ *                                    kv_indices_capacity are not written)
+ * held = held_blocks[b] (NULL: the rows of block_pool hold everything, held = pool_width).  Blocks taken from
+ * free_blocks are appended to the request's row of block_pool, held_blocks_out[b] = max(held, blocks now held),
+ * free_head_out[0] = *free_head + blocks taken, free_head_out[1] = blocks that were needed and could not be had
+ * (the free list, or W, was too short): such a block appears as 0 in the table, its tokens get slot -1.
+ * Earlier sequences are served first, so the result depends on nothing but the inputs.
+ * Inputs and outputs must not overlap except block_pool; request_ids must differ from each other when blocks
+ * are taken.  Lengths below 0 count as 0; a request id outside [0, pool_rows) holds no blocks and takes none;
+ * a block id that is negative, or whose slot does not fit 32 bits, gives slot -1.  batch <= 4096.
+ */
+typedef struct xllm_hip_step_args {
+  const int32_t* cached_lens;  /* [batch] */
+  const int32_t* new_lens;     /* [batch], or NULL: q_per_seq each */
+  const int32_t* request_ids;  /* [batch] rows of block_pool, or NULL: sequence b is row b */
+  const int32_t* held_blocks;  /* [batch], or NULL */
+  int32_t* block_pool;         /* [pool_rows, pool_width], rows pool_stride apart */
+  int64_t pool_stride;
+  const int32_t* free_blocks;  /* [num_free], or NULL: nothing is taken */
+  const int32_t* free_head;    /* [1] index of the first free entry; with free_blocks */
+  int32_t num_free;
+  int32_t pool_rows;
+  int32_t pool_width;
+  int32_t batch;
+  int32_t q_per_seq;           /* used when new_lens == NULL; >= 0 */
+  int32_t block_size;
+  int32_t table_width;
+  int32_t positions_int32;     /* nonzero: positions is int32_t*, else int64_t* */
+  int32_t* block_table;        /* [batch, table_width], rows table_stride apart */
+  int64_t table_stride;
+  int32_t* seq_lens;           /* [batch] */
+  int32_t* q_indptr;           /* [batch + 1] */
+  int32_t* slot_mapping;       /* [num_rows] */
+  void* positions;             /* [num_rows] */
+  int64_t num_rows;
+  int32_t* kv_indptr;          /* [batch + 1], or NULL */
+  int32_t* kv_indices;         /* [kv_indices_capacity] */
+  int32_t* kv_last_page_len;   /* [batch] */
+  int64_t kv_indices_capacity;
+  int32_t* held_blocks_out;    /* [batch]; with held_blocks */
+  int32_t* free_head_out;      /* [2]; with held_blocks */
+} xllm_hip_step_args;
+
+int xllm_hip_build_step_indices(const xllm_hip_step_args* args, xllm_hip_stream_t stream);
+
+/*
+ * Ancestor masks and positions of drafted trees.  parents[q_indptr[b] + v] (or parents[b * q_per_seq + v] when
+ * q_indptr == NULL) is the parent of node v of sequence b as an index within the sequence, or -1 for a child of
+ * the context; nodes may come in any order.  For every node, with itself as its first ancestor:
+ *   mask[row][w] bit i = node 64 w + i is an ancestor of the row's node
+ *   positions[a][row]  = base[b] + number of proper ancestors     (base == NULL: 0), the same for every axis a
+ * base is the position of the first token behind the context: its length, or, for multi-axis positions, the
+ * length plus the sequence's offset.  A parent that names no node of the sequence counts as -1; a cycle of
+ * parents ends nowhere: its nodes' masks hold the cycle's nodes (and depth is then meaningless).  A sequence has
+ * at most 64 * mask_words nodes, mask_words <= 8: nodes past that get empty masks, position base[b], and count as
+ * no one's ancestor.  Rows of no sequence are left as they were.
+ */
+int xllm_hip_tree_masks(const int32_t* parents,
+                        const int32_t* q_indptr,
+                        const int32_t* base,
+                        int32_t batch,
+                        int32_t q_per_seq,
+                        int64_t num_rows,
+                        uint64_t* mask,
+                        int64_t mask_stride, /* words between the rows of mask */
+                        int32_t mask_words,
+                        void* positions,     /* may be NULL */
+                        int32_t positions_int32,
+                        int32_t num_axes,
+                        int64_t axis_stride, /* elements between the axes of positions */
+                        xllm_hip_stream_t stream);
+
+/*
+ * xllm_hip_rope_kv_write with positions of several axes (time, height, width of an image or a video): rotation
+ * pair j turns by the table row of the position on its own axis,
+ *   cos = cos_sin_cache[positions[axis(j)][t]][j],   sin = cos_sin_cache[positions[axis(j)][t]][rotary_dim/2 + j].
+ * sections[a] pairs belong to axis a, sum of sections = rotary_dim / 2.  dealt == 0: side by side, axis 0 first.
+ * dealt != 0: in turn, axis(j) = j mod num_axes where j / num_axes < sections[j mod num_axes], else 0.
+ * args->positions is [num_axes, num_tokens] with axis_stride elements between the axes; everything else of args,
+ * the cache and slot_mapping as in xllm_hip_rope_kv_write (with equal positions on every axis the two calls
+ * compute the same).
+ */
+typedef struct xllm_hip_mrope {
+  int32_t num_axes;  /* 1 .. 4 */
+  int32_t sections[4];
+  int32_t dealt;
+  int64_t axis_stride;
+} xllm_hip_mrope;
+
+int xllm_hip_mrope_kv_write(const xllm_hip_rope_args* args,
+                            const xllm_hip_mrope* axes,
+                            const xllm_hip_kv_cache* cache,
+                            const int32_t* slot_mapping,
+                            xllm_hip_stream_t stream);
+
+/*
+ * Paged attention of drafted trees: xllm_hip_paged_decode with the causal order among a sequence's query tokens
+ * replaced by a mask.  Token j of sequence b (row q_indptr[b] + j, or b * q_per_seq + j; n_b of them, the last n_b
+ * tokens of the kv length L_b) sees
+ *   the keys t < L_b - n_b, and the keys t = L_b - n_b + u, 0 <= u < n_b, with bit u % 64 of tree_mask[row][u / 64] set
+ * (bits past mask_words count as clear).  The mask need not be a tree's: any bits are served.  What a row does not
+ * see takes no part in it whatever it holds (NaN and infinities included); a row that sees nothing yields zeros and
+ * lse = -inf.  args as for xllm_hip_paged_decode: either block-list form, q_indptr or q_per_seq, every cache layout
+ * and type, lse optional; max_seq_len and total_kv_len are hints that only tune how sequences are cut (0 = unknown).
+ * A sliding window (window_left >= 0) and host_plan are refused: XLLM_HIP_UNSUPPORTED.  mask_words <= 8; q_per_seq
+ * <= 512 is the largest n_b; tokens past it are ignored.
+ * `workspace` (256-byte aligned, xllm_hip_tree_attention_workspace_bytes) holds the partial results of sequences that
+ * were cut: written and read within the call, nothing is kept from one call to the next.  One call at a time may
+ * use it.
+ */
+size_t xllm_hip_tree_attention_workspace_bytes(int32_t batch,
+                                               int32_t q_per_seq,
+                                               int32_t num_q_heads,
+                                               int32_t num_kv_heads,
+                                               int32_t head_dim);
+int xllm_hip_tree_attention(const xllm_hip_kv_cache* cache,
+                            const xllm_hip_decode_args* args,
+                            const uint64_t* tree_mask,
+                            int64_t mask_stride, /* words between the rows of tree_mask */
+                            int32_t mask_words,
+                            void* workspace,
+                            size_t workspace_bytes,
+                            xllm_hip_stream_t stream);
+
+/*
+ * The cache rows of the accepted path moved to the front of the drafted range, for one layer's cache: with
+ * c = cached_lens[b] (the length before the draft), every row read before any is written,
+ *   token c + i  <-  token c + accepted[b][i]      for i < min(num_accepted[b], path_width),
+ * K, V and, for a quantised cache, their scales, verbatim.  accepted rows are accepted_stride apart; an entry
+ * below 0, or one whose source or destination block lies outside the table row or the cache, moves nothing.
+ * new_lens[b] = c + min(num_accepted[b], path_width) if new_lens is not NULL.  Sequences must not share the blocks of
+ * their drafted ranges.  path_width <= 1024; num_accepted below 0 counts as 0.
+ */
+int xllm_hip_move_accepted_tokens(const xllm_hip_kv_cache* cache,
+                                  const int32_t* block_table,
+                                  int64_t block_table_stride,
+                                  int32_t max_blocks_per_seq,
+                                  const int32_t* cached_lens,
+                                  const int32_t* accepted,
+                                  int64_t accepted_stride,
+                                  int32_t path_width,
+                                  const int32_t* num_accepted,
+                                  int32_t batch,
+                                  int32_t* new_lens,
+                                  xllm_hip_stream_t stream);
+
 /* XLLM_HIP_ABI_VERSION the library was built with. */
 int xllm_hip_abi_version(void);
 

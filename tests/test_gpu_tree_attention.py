@@ -1,0 +1,356 @@
+"""Paged attention of drafted trees on the GPU against the 64-bit oracle, through the public entry point.
+
+Bounds.  With u = half a step of the queries' type (torch.finfo.eps / 2): the weights and the output are rounded to
+that type once each, so an element may be off by 2 u sum_t p_t |v_t|.  A score is off by d = (D + 8) 2^-24 times the
+largest sum_d |q_d k_d| (float accumulation) and, over an int8 cache, by 2^-16 max|q| sum_d |k_d| more (the kernels may
+hold the queries as 16-bit fixed point); a relative error of at most 2 d follows for the quotient.  Sums of L positive
+floats add L 2^-23, exponentials and logarithms 2^-17."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged_kv_oracle as orc
+from oracle import tree_step_oracle as tro
+from xllm_wxh_amd import _lib, ops
+
+from helpers import TORCH_KV_DTYPE, TORCH_Q_DTYPE, make_tables
+
+pytestmark = pytest.mark.gpu
+
+
+def tree_parents(rng, counts):
+    return np.concatenate([np.array([-1 if j == 0 else int(rng.integers(-1, j)) for j in range(n)], np.int64) for n in counts])
+
+
+class TreeCase:
+    """One problem: host copies for the oracle, device tensors for the call."""
+
+    def __init__(self, counts, lens, Hq, Hkv, D, bs, q="bf16", kv="bf16", layout="HND", mask="tree", words=None, seed=0,
+                 std=1.0, device="cuda"):
+        rng = np.random.default_rng(seed)
+        self.counts, self.lens = list(counts), np.asarray(lens, np.int32)
+        self.Hq, self.Hkv, self.D, self.bs, self.layout, self.q_kind, self.kv = Hq, Hkv, D, bs, layout, q, kv
+        self.q_indptr = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        rows = int(self.q_indptr[-1])
+        words = words or max(1, -(-max(counts) // 64))
+        if mask == "tree":
+            self.mask, _ = tro.tree_masks(tree_parents(rng, counts), self.q_indptr, None, words)
+        elif mask == "random":
+            self.mask = rng.integers(0, 2 ** 64, size=(rows, words), dtype=np.uint64)
+        elif mask == "none":
+            self.mask = np.zeros((rows, words), np.uint64)
+        else:
+            self.mask = np.full((rows, words), 2 ** 64 - 1, np.uint64)
+        self.table, nb = make_tables(len(lens), bs, self.lens, seed)
+        g = torch.Generator().manual_seed(seed)
+        shape = (nb, Hkv, bs, D)
+        kf, vf = torch.randn(shape, generator=g) * std, torch.randn(shape, generator=g)
+        if kv in ("fp8", "int8"):
+            qk, sk = orc.quantize_per_token_head(kf.numpy(), kv)
+            qv, sv = orc.quantize_per_token_head(vf.numpy(), kv)
+            self.k_ref, self.v_ref = orc.dequantize(qk, sk, kv), orc.dequantize(qv, sv, kv)
+            kc = torch.from_numpy(qk.view(np.uint8)).view(TORCH_KV_DTYPE[kv])
+            vc = torch.from_numpy(qv.view(np.uint8)).view(TORCH_KV_DTYPE[kv])
+            ks, vs = torch.from_numpy(sk), torch.from_numpy(sv)
+        else:
+            kc, vc, ks, vs = kf.to(TORCH_KV_DTYPE[kv]), vf.to(TORCH_KV_DTYPE[kv]), None, None
+            self.k_ref, self.v_ref = kc.float().numpy(), vc.float().numpy()
+        qt = torch.randn(rows, Hq, D, generator=g).to(TORCH_Q_DTYPE[q])
+        self.q_ref = qt.float().numpy()
+        self.scale = 1.0 / math.sqrt(D)
+        if layout == "NHD":
+            kc, vc = kc.permute(0, 2, 1, 3).contiguous(), vc.permute(0, 2, 1, 3).contiguous()
+            if ks is not None:
+                ks, vs = ks.permute(0, 2, 1).contiguous(), vs.permute(0, 2, 1).contiguous()
+        to = lambda t: None if t is None else t.to(device)  # noqa: E731
+        self.k, self.v, self.ks, self.vs, self.q = to(kc), to(vc), to(ks), to(vs), to(qt)
+        self.d_mask = to(torch.from_numpy(self.mask.view(np.int64)))
+        self.d_table, self.d_lens, self.d_indptr = (to(torch.from_numpy(np.ascontiguousarray(x))) for x in
+                                                     (self.table, self.lens, self.q_indptr))
+
+    def run(self, **kw):
+        out = torch.full_like(self.q, float("nan"))
+        lse = torch.full((self.q.size(0), self.Hq), float("nan"), dtype=torch.float32, device=self.q.device)
+        kw.setdefault("q_indptr", self.d_indptr)
+        ops.batch_tree_decode(self.q, self.k, self.v, out, kw.pop("table", self.d_table), kw.pop("lens", self.d_lens), self.d_mask,
+                              scale=self.scale, q_per_seq=max(self.counts), output_lse=lse, k_cache_quant_scale=self.ks,
+                              v_cache_quant_scale=self.vs, kv_layout=self.layout, **kw)
+        torch.cuda.synchronize()
+        return out, lse
+
+    def rows(self, ref):
+        got = []
+        for b, n in enumerate(self.lens):
+            pos = np.arange(int(n))
+            got.append(ref[self.table[b, pos // self.bs], :, pos % self.bs])
+        return got
+
+    def oracle(self):
+        return tro.tree_attention(self.q_ref, self.rows(self.k_ref), self.rows(self.v_ref), self.q_indptr, self.lens, self.mask,
+                                  self.scale)
+
+    def check(self, out, lse, ref=None):
+        want, want_lse, absv, dots, ks = ref or self.oracle()
+        L = int(self.lens.max())
+        u = torch.finfo(TORCH_Q_DTYPE[self.q_kind]).eps / 2
+        d = dots * (self.D + 8) * 2.0 ** -24
+        if self.kv == "int8":
+            d = d + ks * np.abs(self.q_ref).max(-1) * 2.0 ** -16
+        sums = (L + 64) * 2.0 ** -23 + 2.0 ** -17
+        tol = absv * (2 * d[..., None] + 2 * u + sums) + 1e-30
+        got = out.float().cpu().numpy().astype(np.float64)
+        assert np.isfinite(got).all()
+        worst = np.abs(got - want) / tol
+        assert worst.max() <= 1.0, "out is %.3g of its bound off at %s" % (worst.max(), np.unravel_index(worst.argmax(), worst.shape))
+        got_lse = lse.cpu().numpy().astype(np.float64)
+        fin = np.isfinite(want_lse)
+        assert np.array_equal(fin, np.isfinite(got_lse)) and np.all(got_lse[~fin] == -np.inf)
+        tol_lse = (d + sums) / math.log(2.0) + 2.0 ** -20 * np.abs(np.where(fin, want_lse, 0.0))
+        assert np.all(np.abs(got_lse[fin] - want_lse[fin]) <= tol_lse[fin])
+
+
+SHAPES = [
+    # counts, lens, Hq, Hkv, D, bs
+    ([1], [1], 4, 2, 64, 32),                                  # one token, nothing but itself
+    ([1, 1], [17, 300], 32, 8, 128, 16),                       # plain decode
+    ([8, 8, 8], [8, 40, 311], 14, 2, 64, 32),                  # a tree without context; 56 rows to a kv head
+    ([5, 1, 13, 2], [64, 33, 500, 130], 8, 2, 128, 16),        # ragged trees
+    ([61, 30], [700, 61], 16, 2, 128, 128),                    # 488 rows to a kv head
+    ([3, 17], [129, 250], 4, 2, 256, 16),
+    ([70], [200], 2, 1, 128, 64),                              # two words to a mask
+]
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "int8"])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_tree_attention_matches_oracle(gpu, shape, kv):
+    counts, lens, Hq, Hkv, D, bs = SHAPES[shape]
+    print("case tree_attention", shape, kv, flush=True)
+    c = TreeCase(counts, lens, Hq, Hkv, D, bs, kv=kv, seed=shape)
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("q,kv", [("fp16", "fp16"), ("fp16", "int8"), ("fp16", "fp8"), ("fp32", "fp32"), ("fp32", "bf16"), ("bf16", "fp16")])
+@pytest.mark.parametrize("D,bs", [(64, 32), (128, 16), (256, 16)])
+def test_other_types_nhd(gpu, q, kv, D, bs):
+    print("case tree types", q, kv, D, flush=True)
+    c = TreeCase([9, 4], [77, 210], 8, 2, D, bs, q=q, kv=kv, layout="NHD", seed=3)
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8", "fp8"])
+@pytest.mark.parametrize("layout", ["HND", "NHD"])
+def test_nhd_and_large_trees(gpu, kv, layout):
+    print("case tree layout", kv, layout, flush=True)
+    c = TreeCase([37, 64, 20], [333, 128, 20], 16, 4, 128, 32, kv=kv, layout=layout, seed=4)
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("D,bs,kv", [(80, 16, "bf16"), (128, 24, "bf16"), (64, 16, "int8"), (128, 8, "fp8"), (96, 5, "fp32")])
+def test_shapes_off_the_matrix_path(gpu, D, bs, kv):
+    print("case tree generic", D, bs, kv, flush=True)
+    c = TreeCase([6, 3], [90, 41], 6, 2, D, bs, kv=kv, q="fp32" if kv == "fp32" else "bf16", seed=5)
+    c.check(*c.run())
+
+
+@pytest.mark.parametrize("mask", ["random", "none", "all"])
+@pytest.mark.parametrize("words", [1, 3])
+def test_any_mask_and_rows_that_see_nothing(gpu, mask, words):
+    print("case tree mask", mask, words, flush=True)
+    # the first sequence has no context: with an empty mask its rows see nothing
+    c = TreeCase([12, 40, 130], [12, 100, 190], 8, 2, 128, 16, mask=mask, words=words, seed=6)
+    out, lse = c.run()
+    c.check(out, lse)
+    if mask == "none":
+        assert torch.all(out[:12] == 0) and torch.all(lse[:12] == -math.inf)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "fp8", "int8"])
+@pytest.mark.parametrize("n,Hq,Hkv", [(4, 8, 2), (16, 16, 4), (24, 8, 2), (40, 16, 2)])
+def test_long_sequences_are_cut(gpu, kv, n, Hq, Hkv):
+    print("case tree split", kv, n, Hq, Hkv, flush=True)
+    c = TreeCase([n, n - 1], [4099, 1500], Hq, Hkv, 128, 16, kv=kv, seed=7)
+    ref = c.oracle()
+    for hints in (dict(), dict(max_seq_len=4099, total_kv_len=5599), dict(max_seq_len=5, total_kv_len=5)):
+        c.check(*c.run(**hints), ref=ref)  # (the last are a captured graph's stale ones)
+
+
+def test_csr_form_uniform_rows_and_strides(gpu):
+    c = TreeCase([7, 7, 7], [100, 7, 260], 8, 2, 128, 16, seed=8)
+    out, lse = c.run(max_seq_len=300)
+    need = (c.lens + c.bs - 1) // c.bs
+    ids = np.concatenate([c.table[b, :need[b]] for b in range(3)]).astype(np.int32)
+    csr = tuple(torch.from_numpy(np.asarray(x, np.int32)).to(gpu) for x in
+                (np.concatenate([[0], np.cumsum(need)]), ids, (c.lens - 1) % c.bs + 1))
+    out2, lse2 = c.run(table=None, lens=None, csr=csr, max_seq_len=300)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+    out3, lse3 = c.run(q_indptr=None, max_seq_len=300)  # 7 rows each, without the offsets
+    assert torch.equal(out, out3) and torch.equal(lse, lse3)
+    # token strides, mask rows and table rows wider than they need be
+    rows = c.q.size(0)
+    q = torch.randn(rows, 10, 128, device=gpu).to(torch.bfloat16)
+    q[:, 1:9] = c.q
+    wide = torch.full((rows, 10, 128), 5.0, device=gpu, dtype=torch.bfloat16)
+    mask = torch.full((rows, 3), -1, dtype=torch.int64, device=gpu)
+    mask[:, 0] = c.d_mask[:, 0]
+    table = torch.full((3, c.table.shape[1] + 3), 2 ** 30, dtype=torch.int32, device=gpu)
+    table[:, :c.table.shape[1]] = c.d_table
+    ops.batch_tree_decode(q[:, 1:9], c.k, c.v, wide[:, 1:9], table[:, :c.table.shape[1]], c.d_lens, mask[:, :1], scale=c.scale,
+                          q_indptr=c.d_indptr, q_per_seq=7, max_seq_len=300)
+    assert torch.equal(wide[:, 1:9], out) and torch.all(wide[:, 0] == 5.0) and torch.all(wide[:, 9] == 5.0)
+
+
+def test_rows_behind_the_last_sequence_and_empty_sequences(gpu):
+    c = TreeCase([5, 6], [50, 90], 8, 2, 128, 16, seed=9)
+    out, _ = c.run()
+    pad = 4
+    q = torch.cat([c.q, torch.full((pad, 8, 128), float("nan"), device=gpu, dtype=torch.bfloat16)])
+    o = torch.full_like(q, 3.0)
+    lse = torch.full((q.size(0), 8), 3.0, device=gpu)
+    mask = torch.cat([c.d_mask, torch.full((pad, 1), -1, dtype=torch.int64, device=gpu)])
+    # two sequences without query tokens, one of them without length, between and behind the others
+    indptr = torch.tensor([0, 5, 5, 11, 11], dtype=torch.int32, device=gpu)
+    lens = torch.tensor([50, 0, 90, 30], dtype=torch.int32, device=gpu)
+    table = torch.stack([c.d_table[0], torch.full_like(c.d_table[0], -7), c.d_table[1], torch.full_like(c.d_table[0], 2 ** 30)])
+    ops.batch_tree_decode(q, c.k, c.v, o, table, lens, mask, scale=c.scale, q_indptr=indptr, q_per_seq=6, output_lse=lse)
+    assert torch.equal(o[:11], out)
+    assert torch.all(o[11:] == 3.0) and torch.all(lse[11:] == 3.0)
+    # query tokens of a sequence of length 0, and more of them than its length
+    lens = torch.tensor([0, 0, 3, 0], dtype=torch.int32, device=gpu)
+    ops.batch_tree_decode(q, c.k, c.v, o, table, lens, mask, scale=c.scale, q_indptr=indptr, q_per_seq=6, output_lse=lse)
+    assert torch.all(o[:5] == 0) and torch.all(lse[:5] == -math.inf) and torch.isfinite(o[5:11]).all()
+
+
+BAD = {"bf16": [float("nan"), float("inf"), -float("inf")], "fp16": [float("nan"), float("inf"), -float("inf")], "fp8": [float("nan")]}
+
+
+@pytest.mark.parametrize("kv,q", [("bf16", "bf16"), ("fp16", "fp16"), ("fp8", "bf16")])
+@pytest.mark.parametrize("n,Hq,Hkv,D,bs", [(6, 8, 2, 128, 16), (24, 8, 2, 128, 16), (50, 16, 2, 128, 32), (6, 8, 2, 64, 32), (6, 4, 2, 256, 16)])
+def test_what_a_row_does_not_see_may_hold_anything(gpu, kv, q, n, Hq, Hkv, D, bs):
+    print("case tree poison", kv, n, D, flush=True)
+    c = TreeCase([n], [3 * n + 41], Hq, Hkv, D, bs, q=q, kv=kv, seed=10)
+    L = int(c.lens[0])
+    out, lse = c.run()
+    # node `victim`: some rows see it, others do not; slots past the length as well
+    victim = n // 2
+    sees = np.array([(int(m) >> victim) & 1 for m in c.mask[:, 0]], bool)
+    assert sees.any() and not sees.all()
+    tok = L - n + victim
+    places = [(int(c.table[0, tok // bs]), tok % bs)] + [(int(c.table[0, t // bs]), t % bs) for t in range(L, c.table.shape[1] * bs)]
+    for what in BAD[kv]:
+        for cache in (c.k, c.v):
+            raw = cache.clone()
+            for blk, slot in places:
+                row = torch.full((Hkv, D), what, device=gpu).to(TORCH_KV_DTYPE[kv])
+                if kv == "fp8":
+                    cache.view(torch.uint8)[blk, :, slot] = row.view(torch.uint8)
+                else:
+                    cache[blk, :, slot] = row
+            got, got_lse = c.run()
+            blind = torch.from_numpy(~sees).to(gpu)
+            assert torch.isfinite(got[blind].float()).all(), (what, cache is c.v)
+            u = torch.finfo(TORCH_Q_DTYPE[q]).eps
+            assert torch.allclose(got[blind].float(), out[blind].float(), rtol=u, atol=u)
+            assert torch.allclose(got_lse[blind], lse[blind], rtol=1e-5, atol=1e-5)
+            if cache is c.v or what != what:
+                assert not torch.isfinite(got[~blind].float()).any(), (what, cache is c.v)
+            if kv == "fp8":
+                cache.view(torch.uint8).copy_(raw.view(torch.uint8))
+            else:
+                cache.copy_(raw)
+
+
+def test_nan_and_infinite_scales_in_unseen_places(gpu):
+    c = TreeCase([6], [60], 8, 2, 128, 16, kv="int8", seed=11)
+    out, lse = c.run()
+    sees = np.array([(int(m) >> 3) & 1 for m in c.mask[:, 0]], bool)
+    blind = torch.from_numpy(~sees).to(gpu)
+    tok = 60 - 6 + 3
+    blk, slot = int(c.table[0, tok // 16]), tok % 16
+    for what in (float("nan"), float("inf")):
+        for scales in (c.ks, c.vs):
+            keep = scales[blk, :, slot].clone()
+            scales[blk, :, slot] = what
+            got, got_lse = c.run()
+            assert torch.allclose(got[blind].float(), out[blind].float(), rtol=2 ** -7, atol=2 ** -7)
+            assert torch.allclose(got_lse[blind], lse[blind], rtol=1e-5, atol=1e-5)
+            scales[blk, :, slot] = keep
+
+
+def test_captured_and_replayed_with_new_lengths(gpu):
+    c = TreeCase([9, 9], [900, 700], 16, 4, 128, 16, seed=12)
+    lens, out = c.d_lens.clone(), torch.zeros_like(c.q)
+    call = lambda o, n: ops.batch_tree_decode(c.q, c.k, c.v, o, c.d_table, n, c.d_mask, scale=c.scale, q_per_seq=9)  # noqa: E731
+    call(out, lens)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):  # two graphs, which must not share their partial results
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(out, lens)
+        graphs.append(g)
+    for a, b in ((900, 700), (9, 350), (899, 9), (64, 65)):
+        lens.copy_(torch.tensor([a, b], dtype=torch.int32, device=gpu))
+        want = torch.empty_like(out)
+        call(want, lens)
+        for g in graphs:
+            out.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want), (a, b)
+
+
+def test_two_streams_at_once(gpu):
+    cases = [TreeCase([12], [3000 + 64 * i], 16, 4, 128, 16, seed=13 + i) for i in range(2)]
+    want = [c.run()[0] for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = [torch.zeros_like(c.q) for c in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for c, s, o in zip(cases, streams, outs):
+            with torch.cuda.stream(s):
+                ops.batch_tree_decode(c.q, c.k, c.v, o, c.d_table, c.d_lens, c.d_mask, scale=c.scale, q_indptr=c.d_indptr, q_per_seq=12)
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
+
+
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+def test_offsets_past_32_bits(gpu, kv):
+    """Blocks more than 2^32 bytes (and, for bf16, 2^31 elements) into the cache."""
+    Hkv, bs, D = 8, 128, 128
+    per = Hkv * bs * D
+    nb = (2 ** 32 + 2 ** 28) // per
+    small = TreeCase([5], [400], 16, Hkv, D, bs, kv=kv, seed=15)
+    big = [torch.empty(nb, Hkv, bs, D, dtype=TORCH_KV_DTYPE[kv], device=gpu) for _ in range(2)]
+    scales = [torch.empty(nb, Hkv, bs, device=gpu) for _ in range(2)] if kv == "int8" else [None, None]
+    table = small.d_table.clone()
+    for i, blk in enumerate(small.table[0]):
+        far = nb - 1 - 3 * i
+        table[0, i] = far
+        for dst, src in zip(big, (small.k, small.v)):
+            dst[far] = src[int(blk)]
+        if kv == "int8":
+            for dst, src in zip(scales, (small.ks, small.vs)):
+                dst[far] = src[int(blk)]
+    want, _ = small.run()
+    out = torch.zeros_like(small.q)
+    ops.batch_tree_decode(small.q, big[0], big[1], out, table, small.d_lens, small.d_mask, scale=small.scale, q_per_seq=5,
+                          k_cache_quant_scale=scales[0], v_cache_quant_scale=scales[1])
+    assert torch.equal(out, want)
+
+
+def test_with_causal_masks_it_is_the_verify_step(gpu):
+    """A chain of drafts is the causal order: the decode path's own verify step gives the same."""
+    n = 4
+    c = TreeCase([n, n], [500, 77], 16, 4, 128, 16, mask="all", seed=16)
+    c.mask[:] = np.array([[(1 << (j + 1)) - 1] for j in range(n)] * 2, np.uint64)
+    c.d_mask.copy_(torch.from_numpy(c.mask.view(np.int64)))
+    out, _ = c.run()
+    want = torch.zeros_like(out)
+    ops.batch_decode(c.q, c.k, want, c.d_table, c.d_lens, c.v, scale=c.scale, q_per_seq=n)
+    # both within their rounding of the same value: weights and output, half a step each, on both sides
+    assert float((out.float() - want.float()).abs().max()) <= 4 * 2.0 ** -8 * float(c.v.float().abs().max())
+    c.check(out, c.run()[1])

@@ -50,6 +50,12 @@ EXPORTED_SYMBOLS = (
     "xllm_hip_swap_blocks",
     "xllm_hip_copy_blocks",
     "xllm_hip_gather_from_cache",
+    "xllm_hip_build_step_indices",
+    "xllm_hip_tree_masks",
+    "xllm_hip_mrope_kv_write",
+    "xllm_hip_tree_attention_workspace_bytes",
+    "xllm_hip_tree_attention",
+    "xllm_hip_move_accepted_tokens",
     "xllm_hip_set_option",
     "xllm_hip_get_option",
     "xllm_hip_last_error",
@@ -136,6 +142,53 @@ class RopeArgs(ctypes.Structure):
     ]
 
 
+class StepArgs(ctypes.Structure):
+    """struct xllm_hip_step_args"""
+
+    _fields_ = [
+        ("cached_lens", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("request_ids", ctypes.c_void_p),
+        ("held_blocks", ctypes.c_void_p),
+        ("block_pool", ctypes.c_void_p),
+        ("pool_stride", ctypes.c_int64),
+        ("free_blocks", ctypes.c_void_p),
+        ("free_head", ctypes.c_void_p),
+        ("num_free", ctypes.c_int32),
+        ("pool_rows", ctypes.c_int32),
+        ("pool_width", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("q_per_seq", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("table_width", ctypes.c_int32),
+        ("positions_int32", ctypes.c_int32),
+        ("block_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("seq_lens", ctypes.c_void_p),
+        ("q_indptr", ctypes.c_void_p),
+        ("slot_mapping", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("num_rows", ctypes.c_int64),
+        ("kv_indptr", ctypes.c_void_p),
+        ("kv_indices", ctypes.c_void_p),
+        ("kv_last_page_len", ctypes.c_void_p),
+        ("kv_indices_capacity", ctypes.c_int64),
+        ("held_blocks_out", ctypes.c_void_p),
+        ("free_head_out", ctypes.c_void_p),
+    ]
+
+
+class Mrope(ctypes.Structure):
+    """struct xllm_hip_mrope"""
+
+    _fields_ = [
+        ("num_axes", ctypes.c_int32),
+        ("sections", ctypes.c_int32 * 4),
+        ("dealt", ctypes.c_int32),
+        ("axis_stride", ctypes.c_int64),
+    ]
+
+
 class XllmHipError(RuntimeError):
     def __init__(self, status, message):
         self.status = status
@@ -194,6 +247,18 @@ def load():
     lib.xllm_hip_gather_from_cache.argtypes = [P(KvCacheDesc), vp, vp, i32, i64, i64, vp, vp, vp, vp, i64, i32, i32,
                                                i32, i32, vp]
     lib.xllm_hip_gather_from_cache.restype = ctypes.c_int
+    lib.xllm_hip_build_step_indices.argtypes = [P(StepArgs), vp]
+    lib.xllm_hip_build_step_indices.restype = ctypes.c_int
+    lib.xllm_hip_tree_masks.argtypes = [vp, vp, vp, i32, i32, i64, vp, i64, i32, vp, i32, i32, i64, vp]
+    lib.xllm_hip_tree_masks.restype = ctypes.c_int
+    lib.xllm_hip_mrope_kv_write.argtypes = [P(RopeArgs), P(Mrope), P(KvCacheDesc), vp, vp]
+    lib.xllm_hip_mrope_kv_write.restype = ctypes.c_int
+    lib.xllm_hip_tree_attention_workspace_bytes.argtypes = [i32, i32, i32, i32, i32]
+    lib.xllm_hip_tree_attention_workspace_bytes.restype = ctypes.c_size_t
+    lib.xllm_hip_tree_attention.argtypes = [P(KvCacheDesc), P(DecodeArgs), vp, i64, i32, vp, ctypes.c_size_t, vp]
+    lib.xllm_hip_tree_attention.restype = ctypes.c_int
+    lib.xllm_hip_move_accepted_tokens.argtypes = [P(KvCacheDesc), vp, i64, i32, vp, vp, i64, i32, vp, i32, vp, vp]
+    lib.xllm_hip_move_accepted_tokens.restype = ctypes.c_int
     lib.xllm_hip_set_option.argtypes = [i32, i64]
     lib.xllm_hip_set_option.restype = ctypes.c_int
     lib.xllm_hip_get_option.argtypes = [i32]
