@@ -11,6 +11,7 @@
 #include "device_utils.h"
 #include "host_utils.h"
 #include "tree_generic.h"
+#include "tree_mfma.h"
 #include "tree_params.h"
 
 #include <math.h>
@@ -56,6 +57,121 @@ static void launch_tree_generic(int kv_dt, const TreeParams& p, unsigned grid, h
     default:
       tree_generic_kernel<Q_DT, XLLM_HIP_INT8><<<grid, 64, 0, st>>>(p);
       break;
+  }
+}
+
+// How the matrix kernels would run a call; rows_per_item 0: they do not serve it.
+struct TreeForm {
+  int rows_per_item;
+  int tile;
+  int slots;  // workgroups that run at a time on 256 CUs
+};
+
+static TreeForm tree_form(const xllm_hip_kv_cache* c, const xllm_hip_decode_args* a) {
+  TreeForm none{0, 64, 0};
+  const int eb = elem_bytes(c->dtype);
+  const bool quant = c->dtype == XLLM_HIP_FP8_E4M3 || c->dtype == XLLM_HIP_INT8;
+  if (a->q_dtype != XLLM_HIP_BF16 && a->q_dtype != XLLM_HIP_FP16) return none;
+  if (!quant && c->dtype != a->q_dtype) return none;
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return none;
+  // (a wave's load instruction covers rows of one group of 16 tokens, which must lie in one block)
+  if (!is_pow2(c->block_size) || c->block_size < 16) return none;
+  if (!(a->sm_scale >= 0.0f)) return none;  // (the running maximum is taken before the scale)
+  const int64_t vec = 16 / eb, lim = (int64_t)1 << 31;
+  if (c->stride_block % vec != 0 || c->stride_head % vec != 0 || c->stride_slot % vec != 0) return none;
+  if (c->stride_block >= lim || c->stride_slot * c->block_size >= lim) return none;
+  if (quant && (c->scale_stride_block >= lim || c->scale_stride_slot * c->block_size >= lim)) return none;
+  if ((((uintptr_t)c->k_cache | (uintptr_t)c->v_cache | (uintptr_t)a->q | (uintptr_t)a->out) & 15) != 0) return none;
+  if (a->q_token_stride % 8 != 0 || a->out_token_stride % 8 != 0) return none;
+  const int64_t rows = (int64_t)a->q_per_seq * (a->num_q_heads / c->num_kv_heads);
+  const int rb = c->head_dim * eb;
+  TreeForm f;
+  f.rows_per_item = rows <= 32 ? 32 : (rows <= 64 || c->head_dim == 256) ? 64 : 128;
+  f.tile = rb >= 256 ? 64 : 128;
+  f.slots = rb == 512 ? 256 : 512;
+  return f;
+}
+
+// Tokens per chunk and chunks per sequence (at most p.slots of them on entry).  Without the host's lengths: as many
+// chunks as the workspace holds, of at least kTreeMinChunk tokens.  With them, the cut whose step is predicted to end
+// first, counted in tokens a workgroup gets through (`at_once` of them run together):
+//   nearly equal lengths   rounds of equal items:  ceil(items / at_once) * (chunk + kItemTokens)
+//   ragged lengths         items / at_once * (mean chunk + kItemTokens), and half a chunk until the last one ends
+// plus, where sequences are cut, the merge's launch and the partial results, written once and read once (a row's 4
+// bytes per element against the 2 * eb a cached token takes, shared by the whole GPU).
+static void choose_chunks(const xllm_hip_decode_args* a, const TreeForm& form, int eb, TreeParams& p) {
+  constexpr int64_t kItemTokens = 64;
+  constexpr int64_t kMergeTokens = 128;
+  auto whole = [&](int64_t tokens) { return (tokens + p.tile - 1) / p.tile * p.tile; };
+  const int64_t longest = a->max_seq_len;
+  if (longest <= 0 || form.rows_per_item == 0) {
+    p.chunk = (int32_t)whole(kTreeMinChunk);
+    if (longest > 0) {  // (chunk slots no sequence reaches are not launched)
+      const int64_t most = (longest + p.chunk - 1) / p.chunk;
+      if (most < p.slots) p.slots = (int32_t)most;
+    }
+    return;
+  }
+  int64_t total = a->total_kv_len;
+  if (total <= 0 || total > longest * p.batch) total = longest * p.batch;
+  const bool equal = longest * p.batch * 4 <= total * 5;
+  const int64_t lanes = (int64_t)p.num_kv_heads * p.row_groups;
+  const int64_t item_rows = (int64_t)p.n * p.group < form.rows_per_item ? (int64_t)p.n * p.group : form.rows_per_item;
+  double best = 0.0;
+  int best_cut = 0;
+  for (int cut = 1; cut <= p.slots; ++cut) {
+    const int64_t chunk = whole((longest + cut - 1) / cut);
+    if (cut > 1 && chunk < kTreeMinChunk) break;
+    double t;
+    if (equal) {
+      const int64_t items = lanes * p.batch * ((longest + chunk - 1) / chunk);
+      t = (double)((items + form.slots - 1) / form.slots) * (double)(chunk + kItemTokens);
+      if (cut > 1) t += (double)items * item_rows * 4.0 / eb / form.slots;
+    } else {
+      const double items = (double)lanes * ((double)total / (double)chunk + 0.5 * p.batch);
+      t = ((double)lanes * (double)total + items * kItemTokens) / form.slots + 0.5 * (double)chunk;
+      if (cut > 1) t += items * item_rows * 4.0 / eb / form.slots;
+    }
+    if (cut > 1) t += kMergeTokens;
+    if (best_cut == 0 || t < best) {
+      best = t;
+      best_cut = cut;
+    }
+  }
+  p.chunk = (int32_t)whole((longest + best_cut - 1) / best_cut);
+  p.slots = best_cut;
+}
+
+template <int QT, int KV, int D>
+static void launch_tree_mfma_d(int rows_per_item, const TreeParams& p, unsigned grid, hipStream_t st) {
+  if (rows_per_item == 32) {
+    tree_mfma_kernel<QT, KV, D, 1, 2><<<grid, 256, 0, st>>>(p);
+  } else if (rows_per_item == 64) {
+    tree_mfma_kernel<QT, KV, D, 1, 1><<<grid, 256, 0, st>>>(p);
+  } else {
+    if constexpr (D <= 128) tree_mfma_kernel<QT, KV, D, 2, 1><<<grid, 256, 0, st>>>(p);
+  }
+}
+
+template <int QT, int KV>
+static void launch_tree_mfma_kv(int rows_per_item, const TreeParams& p, unsigned grid, hipStream_t st) {
+  if (p.head_dim == 64) {
+    launch_tree_mfma_d<QT, KV, 64>(rows_per_item, p, grid, st);
+  } else if (p.head_dim == 128) {
+    launch_tree_mfma_d<QT, KV, 128>(rows_per_item, p, grid, st);
+  } else {
+    launch_tree_mfma_d<QT, KV, 256>(rows_per_item, p, grid, st);
+  }
+}
+
+template <int QT>
+static void launch_tree_mfma(int kv_dt, int rows_per_item, const TreeParams& p, unsigned grid, hipStream_t st) {
+  if (kv_dt == XLLM_HIP_FP8_E4M3) {
+    launch_tree_mfma_kv<QT, XLLM_HIP_FP8_E4M3>(rows_per_item, p, grid, st);
+  } else if (kv_dt == XLLM_HIP_INT8) {
+    launch_tree_mfma_kv<QT, XLLM_HIP_INT8>(rows_per_item, p, grid, st);
+  } else {
+    launch_tree_mfma_kv<QT, QT>(rows_per_item, p, grid, st);
   }
 }
 
@@ -171,24 +287,30 @@ extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
     p.partial_lse = (float*)workspace;
     p.partial_out = (float*)((uint8_t*)workspace + tree_lse_bytes(a->batch, p.n, p.num_q_heads, slots));
   }
-  p.tile = 64;
-  p.chunk = kTreeMinChunk;
-  // Chunk slots no sequence can reach by the host's hint are not launched (a longer sequence than the hint says gets
-  // longer chunks).
-  if (a->max_seq_len > 0) {
-    const int64_t most = ((int64_t)a->max_seq_len + p.chunk - 1) / p.chunk;
-    if (most < p.slots) p.slots = (int32_t)most;
+  const TreeForm form = tree_form(c, a);
+  p.tile = form.tile;
+  const int64_t rows = (int64_t)p.n * p.group;
+  p.row_groups = (int32_t)(form.rows_per_item > 0 ? (rows + form.rows_per_item - 1) / form.rows_per_item : rows);
+  choose_chunks(a, form, elem_bytes(c->dtype), p);
+  int64_t items = (int64_t)p.batch * p.slots * p.num_kv_heads * p.row_groups;
+  if (form.rows_per_item > 0 && p.row_groups > 1) {  // whole rounds of the XCDs (see the kernel)
+    items = (items + kTreeXcds * p.row_groups - 1) / (kTreeXcds * p.row_groups) * (kTreeXcds * p.row_groups);
   }
-  p.row_groups = p.n * p.group;
-  const int64_t items = (int64_t)p.batch * p.slots * p.num_kv_heads * p.row_groups;
   XLLM_HIP_REQUIRE(items <= 0x7fffffff, "too many work items: %lld", (long long)items);
   hipStream_t st = (hipStream_t)stream;
-  if (p.q_dtype == XLLM_HIP_BF16) {
-    launch_tree_generic<XLLM_HIP_BF16>(c->dtype, p, (unsigned)items, st);
+  const unsigned grid = (unsigned)items;
+  if (form.rows_per_item > 0) {
+    if (p.q_dtype == XLLM_HIP_BF16) {
+      launch_tree_mfma<XLLM_HIP_BF16>(c->dtype, form.rows_per_item, p, grid, st);
+    } else {
+      launch_tree_mfma<XLLM_HIP_FP16>(c->dtype, form.rows_per_item, p, grid, st);
+    }
+  } else if (p.q_dtype == XLLM_HIP_BF16) {
+    launch_tree_generic<XLLM_HIP_BF16>(c->dtype, p, grid, st);
   } else if (p.q_dtype == XLLM_HIP_FP16) {
-    launch_tree_generic<XLLM_HIP_FP16>(c->dtype, p, (unsigned)items, st);
+    launch_tree_generic<XLLM_HIP_FP16>(c->dtype, p, grid, st);
   } else {
-    launch_tree_generic<XLLM_HIP_FP32>(c->dtype, p, (unsigned)items, st);
+    launch_tree_generic<XLLM_HIP_FP32>(c->dtype, p, grid, st);
   }
   int rc = check_launch("tree attention kernel");
   if (rc != XLLM_HIP_OK || p.slots == 1) return rc;

@@ -1,0 +1,683 @@
+// Tree attention on the matrix cores: head_dim 64, 128 and 256, 16-bit queries, 16-bit and 8-bit caches.
+//
+// One workgroup of four waves per (sequence chunk, kv head, group of query rows); query row r = j * group + gq (token
+// j, head gq of the kv head's group).  The products are taken transposed, 16 query rows to a matrix tile,
+//   S^T[t][r]  = sum_d K[t][d] Q[r][d]        A = K from LDS,    B = Q^T in registers
+//   O^T[d][r] += sum_t V[t][d] P[r][t]        A = V^T from LDS,  B = P^T, the softmax weights as S^T left them
+// so that a query row stays in one lane column from the scores to the output, and its running maximum and sum are a
+// lane's own numbers.  K and V go from memory straight into LDS (16 bytes a lane, no registers on the way), the tile
+// after the one in use always in flight; an 8-bit cache stays bytes there — half the LDS traffic — and becomes 16-bit
+// operands in the registers that feed the matrix instructions:
+//   fp8   K to the queries' type, V to fp16, both exact
+//   int8  x ^ 0x80 = x + 128 placed behind 0x64 is the fp16 number 1024 + 128 + x; minus 1152 it is x, exactly
+// With V in fp16 the weights of an 8-bit cache are rounded to 11 bits, those over a bf16 cache to 8.
+//
+// How the waves share an item: 64 rows or 128 rows to a workgroup are 16 or 32 to each wave, which then reads all of
+// the tile; up to 32 rows are two tiles of 16, and two waves share a row tile, taking alternate 32-token pieces.  The
+// second half of such an item's arithmetic is often unused (16 rows or fewer): a step this narrow is bound by memory.
+//
+// Only the last tokens of a sequence are drafted ones, so only the last pieces are masked.  There a row takes from its
+// mask the 32 bits of the piece; scores of unseen tokens are replaced by -inf whatever they were.  An unseen V may
+// hold anything, and 0 * NaN in a matrix product would reach every row, so the V rows of a masked tile are looked
+// through: rows past the length are zeroed, and where another holds a NaN or an infinity the piece is accumulated
+// token by token under each row's own bits.
+#pragma once
+
+#include "decode_mfma.h"
+#include "tree_params.h"
+
+namespace xllm_hip {
+
+constexpr bool tree_quant(int kv) { return kv == XLLM_HIP_FP8_E4M3 || kv == XLLM_HIP_INT8; }
+
+template <int QT, int KV, int D>
+struct TreeShape {
+  static constexpr bool kQuant = tree_quant(KV);
+  static constexpr bool kInt8 = KV == XLLM_HIP_INT8;
+  static constexpr int kEB = kQuant ? 1 : 2;
+  static constexpr int kRB = D * kEB;                  // bytes of a cache row
+  static constexpr int kPPR = kRB / 16;                // 16-byte pieces of a row
+  static constexpr int kRPI = 64 / kPPR;               // rows a load instruction of a wave covers
+  static constexpr int kTT = kRB >= 256 ? 64 : 128;    // tokens per tile
+  static constexpr int kRW = kTT / 4;                  // tokens of a tile that one wave fetches
+  static constexpr int kLoads = kRW / kRPI;            // load instructions a wave needs for them (K; as many for V)
+  static constexpr int kArray = kTT * kRB;             // bytes of a tile's K or V
+  static constexpr int kFactors = 2 * kArray;          // three per-token factors of an 8-bit cache behind them
+  static constexpr int kStage = 2 * kArray + (kQuant ? 3 * kTT * 4 : 0);
+  static constexpr bool kQF16 = QT == XLLM_HIP_FP16;
+  static constexpr bool kKF16 = kQF16 || kInt8;        // type of the first product: fp16, else bf16
+  static constexpr bool kVF16 = kQF16 || kQuant;       // type of the second
+  static constexpr bool kNormQ = kInt8 && !kQF16;      // bf16 queries that become fp16: see init
+  static constexpr int kChunks = D / 32;
+  static constexpr int kDT = D / 16;
+};
+
+// LDS placement: the 16-byte pieces of a row are permuted by an XOR that depends on the row, so that the lanes the LDS
+// serves together (8 of a 16-byte access, 16 of an 8-byte one: 128 bytes) meet all 8 pieces (mod 8):
+//   K: 8 consecutive rows, same piece;   V, 16-bit: 4 rows x 2 pieces;   V, 8-bit: rows r..r+3 and r+16.., same piece.
+// A 64-byte row (head_dim 64, 8-bit) is half a line: there the row's parity is one of the three bits already.
+template <int RB>
+__device__ inline int tree_swz_k(int row) {
+  return RB == 64 ? (row >> 1) & 3 : row & 7;
+}
+template <int RB, bool QUANT>
+__device__ inline int tree_swz_v(int row) {
+  if (!QUANT) return (row & 3) << 1;
+  return RB == 64 ? ((row >> 1) & 1) | (((row >> 4) & 1) << 1) : (row & 3) | (((row >> 4) & 1) << 2);
+}
+
+// Eight bytes of an 8-bit cache as eight 16-bit numbers.
+template <int KV, bool F16>
+__device__ inline u32x4 tree_widen(uint32_t a, uint32_t b) {
+  u32x4 o;
+  const uint32_t in[2] = {a, b};
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    if constexpr (KV == XLLM_HIP_INT8) {
+      static_assert(KV != XLLM_HIP_INT8 || F16, "int8 operands are fp16");
+      const uint32_t t = in[w] ^ 0x80808080u;
+      const f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+      const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, t, 0x04010400u)) - off;
+      const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, t, 0x04030402u)) - off;
+      o[2 * w] = __builtin_bit_cast(uint32_t, lo);
+      o[2 * w + 1] = __builtin_bit_cast(uint32_t, hi);
+    } else if constexpr (F16) {
+      o[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(in[w], 1.0f, false));
+      o[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(in[w], 1.0f, true));
+    } else {
+      o[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)in[w], 1.0f, false));
+      o[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)in[w], 1.0f, true));
+    }
+  }
+  return o;
+}
+
+// Any non-finite value among the 16 bytes?
+template <int KV>
+__device__ inline bool tree_not_finite(u32x4 v) {
+  uint32_t hit = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if constexpr (KV == XLLM_HIP_FP8_E4M3) {
+      // a byte is a NaN if its low seven bits are all set: adding one to them carries into bit 7
+      hit |= ((v[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    } else {
+      const uint32_t e = KV == XLLM_HIP_BF16 ? 0x7f807f80u : 0x7c007c00u;
+      const uint32_t one = KV == XLLM_HIP_BF16 ? 0x00800080u : 0x04000400u;
+      hit |= ((v[w] & e) + one) & 0x80008000u;  // an exponent of all ones carries into the sign's place
+    }
+  }
+  return hit != 0;
+}
+
+// One wave's share of the loads: where its rows lie, and the loads of a tile.
+template <class SH, int KV>
+struct TreeLoader {
+  uint32_t off_k[SH::kLoads], off_v[SH::kLoads];  // byte offset of this lane's piece from the first of the 16 tokens
+  int wave, lane;
+  float sc;  // the scale in flight: lanes 0..31 the K scales of the wave's tokens, 32..63 the V scales
+  uint32_t sc_off;
+
+  __device__ inline void init(const TreeParams& p, int w, int l) {
+    wave = w;
+    lane = l;
+    const int pos = l % SH::kPPR;
+#pragma unroll
+    for (int q = 0; q < SH::kLoads; ++q) {
+      const int rw = q * SH::kRPI + l / SH::kPPR;  // row among the wave's
+      const int row = w * SH::kRW + rw;            // row of the tile
+      const uint32_t at = (uint32_t)((rw & 15) * p.stride_slot) * SH::kEB;
+      off_k[q] = at + ((pos ^ tree_swz_k<SH::kRB>(row)) << 4);
+      off_v[q] = at + ((pos ^ tree_swz_v<SH::kRB, SH::kQuant>(row)) << 4);
+    }
+    sc = 0.0f;
+    sc_off = 0;
+    if (SH::kQuant) sc_off = (uint32_t)((l & 15) * p.sc_stride_slot) * 4;
+  }
+
+  // The block that holds the wave's group g (16 tokens) of the tile at tb, by a scalar load; past the sequence's list
+  // its last block.
+  __device__ static inline int block(const TreeParams& p, const TreeItem& it, int tok) {
+    int bi = tok >> p.log2_bs;
+    bi = bi < it.nblk ? bi : it.nblk - 1;
+    return tree_block(p, ((const __attribute__((address_space(4))) int32_t*)it.ids)[bi]);
+  }
+
+  __device__ inline void issue(const TreeParams& p, const TreeItem& it, int tb, uint8_t* stage) {
+    constexpr int kGroups = SH::kRW / 16;
+    constexpr int kPer = SH::kLoads / kGroups;  // load instructions per group
+    const int first = tb + wave * SH::kRW;
+    uint8_t* kl = stage + wave * (SH::kRW * SH::kRB);
+    uint8_t* vl = kl + SH::kArray;
+    int64_t sbase[kGroups];
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g) {
+      const int tok = first + 16 * g;
+      const int blk = block(p, it, tok);
+      const uint32_t slot = (uint32_t)(tok & (p.block_size - 1));
+      const int64_t elem = (int64_t)((uint64_t)(uint32_t)blk * (uint32_t)p.stride_block) + (int64_t)it.hk * p.stride_head +
+                           (int64_t)(slot * (uint32_t)p.stride_slot);
+      if (SH::kQuant) {
+        sbase[g] = (int64_t)((uint64_t)(uint32_t)blk * (uint32_t)p.sc_stride_block) + (int64_t)it.hk * p.sc_stride_head +
+                   (int64_t)(slot * (uint32_t)p.sc_stride_slot);
+      }
+      const uint8_t* kb = p.k_cache + elem * SH::kEB;
+      const uint8_t* vb = p.v_cache + elem * SH::kEB;
+#pragma unroll
+      for (int q = g * kPer; q < (g + 1) * kPer; ++q) XLLM_HIP_GLOBAL_TO_LDS_16(kb + off_k[q], kl + q * 1024);
+#pragma unroll
+      for (int q = g * kPer; q < (g + 1) * kPer; ++q) XLLM_HIP_GLOBAL_TO_LDS_16(vb + off_v[q], vl + q * 1024);
+    }
+    if constexpr (SH::kQuant) {
+      // lane = (array, token among the wave's, 16 of them twice where there are only 16)
+      const int64_t sb = kGroups > 1 && (lane & 16) != 0 ? sbase[kGroups - 1] : sbase[0];
+      const float* arr = (lane & 32) != 0 ? p.v_scale : p.k_scale;
+      sc = *(const float*)((const uint8_t*)(arr + sb) + sc_off);
+    }
+  }
+
+  // The per-token factors of the tile whose scales have arrived:
+  //   kscl = k_scale * sm_scale * log2 e       x = s * kscl + lv
+  //   lv   = log2 v_scale                      weight 2^(x - max x): the V scale rides in the exponent, so the 16-bit
+  //   rvs  = 1 / v_scale                       weights use their whole range; a weight's share of the sum is w * rvs
+  // A V scale of 0 counts as 2^-100: its tokens keep their share of the sum and add nothing.
+  __device__ inline void factors(const TreeParams& p, uint8_t* stage) const {
+    if constexpr (SH::kQuant) {
+      float* f = (float*)(stage + SH::kFactors);
+      const int i = lane & 31;
+      if (i < SH::kRW) {
+        const int t = wave * SH::kRW + i;
+        if (lane < 32) {
+          f[t] = sc * p.scale_log2;
+        } else {
+          const float vs = sc < 0x1p-100f ? 0x1p-100f : sc;  // (a NaN stays one)
+          f[SH::kTT + t] = __builtin_amdgcn_logf(vs);
+          f[2 * SH::kTT + t] = __builtin_amdgcn_rcpf(vs);
+        }
+      }
+    }
+  }
+
+  // The wave's V rows of a masked tile, landed: zeros over the rows past the length; whether another holds something
+  // that is not finite.
+  __device__ inline bool look_through(int tb, int len, uint8_t* stage) const {
+    bool bad = false;
+    if constexpr (KV != XLLM_HIP_INT8) {
+#pragma unroll
+      for (int q = 0; q < SH::kLoads; ++q) {
+        const int tok = tb + wave * SH::kRW + q * SH::kRPI + lane / SH::kPPR;
+        u32x4* at = (u32x4*)(stage + SH::kArray + wave * (SH::kRW * SH::kRB) + q * 1024 + lane * 16);
+        if (tok >= len) {
+          *at = u32x4{0, 0, 0, 0};
+        } else {
+          bad = bad || tree_not_finite<KV>(*at);
+        }
+      }
+    }
+    return __builtin_amdgcn_ballot_w64(bad) != 0;
+  }
+};
+
+// The lane's query row among the item's, in the row tile that starts at first_row; -1: none.
+__device__ inline int tree_row(const TreeParams& p, const TreeItem& it, int first_row, int lane) {
+  const int row = first_row + (lane & 15);
+  return row < it.n * p.group ? row : -1;
+}
+
+// The mask of the lane's row.
+struct TreeRowMask {
+  const uint64_t* mask;
+  uint64_t word0;
+  int words;  // 0 where the lane has no row
+
+  __device__ inline void init(const TreeParams& p, const TreeItem& it, int first_row, int lane) {
+    const int row = tree_row(p, it, first_row, lane);
+    mask = p.mask + (it.q0 + (row < 0 ? 0 : row) / p.group) * p.mask_stride;
+    words = row < 0 ? 0 : p.mask_words;
+    word0 = row < 0 ? 0 : mask[0];
+  }
+
+  // Bits of the 32 tokens from t0 on that the row sees.
+  __device__ inline uint32_t bits(const TreeItem& it, int t0) const {
+    uint32_t b;
+    const int u = t0 - it.prefix;
+    if (u <= -32) {
+      b = ~0u;
+    } else if (u < 0) {  // the context's last tokens, then the first drafted ones
+      b = (uint32_t)(word0 << -u) | ((1u << -u) - 1u);
+    } else {
+      const int w = u >> 6, s = u & 63;
+      const uint64_t lo = w == 0 ? word0 : (w < words ? mask[w] : 0);
+      uint64_t v = lo >> s;
+      if (s > 32 && w + 1 < words) v |= mask[w + 1] << (64 - s);
+      b = (uint32_t)v;
+    }
+    const int left = it.len - t0;
+    if (left < 32) b &= left > 0 ? (1u << left) - 1u : 0u;
+    return b;
+  }
+};
+
+// 16 query rows of one wave.
+template <class SH, int KV>
+struct TreeRows {
+  typedef typename MmaOps<SH::kKF16>::Op OpK;
+  typedef typename MmaOps<SH::kVF16>::Op OpV;
+  OpK qf[SH::kChunks];
+  f32x4 acc[SH::kDT];
+  float m_run, l_run;
+  float q_scale;          // kNormQ: factor of the row's scores
+  __device__ inline void init(const TreeParams& p, const TreeItem& it, int first_row, int lane) {
+    const int kg = lane >> 4;
+    const int row = tree_row(p, it, first_row, lane);
+    const int r = row < 0 ? 0 : row;
+    const int j = r / p.group;
+    const int64_t token = it.q0 + j;
+    const uint16_t* q = (const uint16_t*)p.q + token * p.q_token_stride + (int64_t)(it.hk * p.group + (r - j * p.group)) * (SH::kDT * 16);
+    q_scale = 1.0f;
+    u32x4 raw[SH::kChunks];
+#pragma unroll
+    for (int c = 0; c < SH::kChunks; ++c) {
+      // elements of chunk c this lane feeds: as the K bytes lie (an 8-bit K piece of 16 elements feeds two chunks)
+      const int at = SH::kQuant ? 64 * (c >> 1) + 16 * kg + 8 * (c & 1) : 32 * c + 8 * kg;
+      raw[c] = u32x4{0, 0, 0, 0};
+      if (row >= 0) raw[c] = *(const u32x4*)(q + at);
+    }
+    if constexpr (SH::kNormQ) {
+      // bf16 queries become fp16: the row is first brought to a largest magnitude in [2^14, 2^15) by a power of two,
+      // exactly, so that neither end of fp16's range cuts into what bf16 holds (elements 2^28 below the largest lose
+      // bits); the scores take the factor back.
+      float top = 0.0f;
+#pragma unroll
+      for (int c = 0; c < SH::kChunks; ++c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf((float)__builtin_bit_cast(bf16x8, raw[c])[e]));
+      }
+      top = kg_max(top);
+      int e2 = (int)((__builtin_bit_cast(uint32_t, top) >> 23) & 0xffu) - 126 - 15;
+      e2 = e2 < -100 ? -100 : (e2 > 100 ? 100 : e2);
+      const float down = __builtin_amdgcn_ldexpf(1.0f, -e2);
+      q_scale = __builtin_amdgcn_ldexpf(1.0f, e2);
+#pragma unroll
+      for (int c = 0; c < SH::kChunks; ++c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qf[c][e] = (_Float16)((float)__builtin_bit_cast(bf16x8, raw[c])[e] * down);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < SH::kChunks; ++c) qf[c] = __builtin_bit_cast(OpK, raw[c]);
+    }
+    m_run = -INFINITY;
+    l_run = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < SH::kDT; ++dt) acc[dt] = f32x4{0, 0, 0, 0};
+  }
+
+  // The scale rides in the FMA that forms the exponent where nothing else needs the scaled score.
+  template <bool MASKED>
+  static constexpr bool kFold = !SH::kQuant && !MASKED;
+
+  // Scores of 32 tokens (s[h][rr]: token 16h + 4kg + rr), scaled and masked, in x (index 4h + rr).
+  template <bool MASKED>
+  __device__ __forceinline__ void scaled(const f32x4 (&s)[2], const f32x4 (&kscl)[2], const f32x4 (&lv)[2], float scale_log2, uint32_t vis,
+                                         int kg, float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v = s[i >> 2][i & 3];
+      if constexpr (SH::kNormQ) v *= q_scale;
+      if constexpr (SH::kQuant) {
+        v = __builtin_fmaf(v, kscl[i >> 2][i & 3], lv[i >> 2][i & 3]);
+      } else if constexpr (!kFold<MASKED>) {
+        v *= scale_log2;
+      }
+      if (MASKED) v = (vis >> (16 * (i >> 2) + 4 * kg + (i & 3))) & 1 ? v : -INFINITY;
+      x[i] = v;
+    }
+  }
+
+  // Scores to weights, in place; returns whether the reference point of some row moved.
+  template <bool MASKED>
+  __device__ __forceinline__ bool weights(float (&x)[8], const f32x4 (&rvs)[2], float scale_log2, uint32_t vis, int kg, float& alpha) {
+    const float neg_inf = -INFINITY;
+    float mt = neg_inf;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mt = fmaxf(mt, x[i]);
+    mt = kg_max(mt);
+    if (kFold<MASKED>) mt *= scale_log2;
+    // The reference point of the exponents follows the running maximum lazily: it moves when a row's maximum has grown
+    // by more than kLazyRescale (in log 2).  Weights up to that are harmless, and the accumulators are seldom rescaled.
+    const float m_top = fmaxf(m_run, mt);
+    const bool moved = __builtin_amdgcn_ballot_w64(m_top > m_run + kLazyRescale) != 0;
+    const float m_new = moved ? m_top : m_run;
+    const float m_safe = m_new == neg_inf ? 0.0f : m_new;
+    alpha = __builtin_amdgcn_exp2f(m_run - m_safe);
+    l_run *= alpha;
+    m_run = m_new;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float e = __builtin_amdgcn_exp2f(kFold<MASKED> ? __builtin_fmaf(x[i], scale_log2, -m_safe) : x[i] - m_safe);
+      x[i] = e;
+      if constexpr (SH::kQuant) {
+        const float share = e * rvs[i >> 2][i & 3];
+        // (an unseen token's scale may be anything: 0 * NaN must not reach the sum)
+        l_run += MASKED ? ((vis >> (16 * (i >> 2) + 4 * kg + (i & 3))) & 1 ? share : 0.0f) : share;
+      } else {
+        l_run += e;
+      }
+    }
+    return moved;
+  }
+
+  __device__ static inline OpV pack(const float (&w)[8]) {
+    typedef MmaOps<SH::kVF16> M;
+    return __builtin_bit_cast(OpV, u32x4{M::pack(w[0], w[1]), M::pack(w[2], w[3]), M::pack(w[4], w[5]), M::pack(w[6], w[7])});
+  }
+};
+
+// RTW: row tiles per wave; TS: waves that share a row tile's tokens (2 with RTW = 1, else 1).
+template <int QT, int KV, int D, int RTW, int TS>
+__global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1 : 2)) tree_mfma_kernel(TreeParams p) {
+  typedef TreeShape<QT, KV, D> SH;
+  static_assert(TS == 1 || (TS == 2 && RTW == 1), "two waves share one row tile at most");
+  constexpr int kRowsPerItem = 16 * RTW * 4 / TS;
+  __shared__ __attribute__((aligned(16))) uint8_t stage0[SH::kStage];
+  __shared__ __attribute__((aligned(16))) uint8_t stage1[SH::kStage];
+  __shared__ int found[2][4];  // per stage and wave: a masked tile's V rows hold something that is not finite
+  static_assert(SH::kDT * 1024 + 512 <= SH::kStage, "the exchange of two waves must fit a stage");
+
+  TreeItem it;
+  int id = blockIdx.x;
+  if (p.row_groups > 1) {
+    // the row groups of one (chunk, kv head) read the same K and V: neighbours on one XCD, whose L2 they share
+    const int on = id / kTreeXcds;
+    id = ((on / p.row_groups) * kTreeXcds + id % kTreeXcds) * p.row_groups + on % p.row_groups;
+  }
+  if (!tree_item(p, id, kRowsPerItem, it)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int mi = lane & 15, kg = lane >> 4;
+  const int tg = TS == 2 ? wave >> 1 : 0;                        // which of the two waves of the row tile
+  const int first_row = it.rg * kRowsPerItem + (TS == 2 ? wave & 1 : wave * RTW) * 16;
+
+  TreeLoader<SH, KV> ld;
+  ld.init(p, wave, lane);
+  const int t0 = it.t_begin;
+  const int iters = it.t_end > t0 ? (it.t_end - t0 + SH::kTT - 1) / SH::kTT : 0;
+  if (iters > 0) ld.issue(p, it, t0, stage0);
+
+  TreeRows<SH, KV> rows[RTW];
+#pragma unroll
+  for (int a = 0; a < RTW; ++a) rows[a].init(p, it, first_row + 16 * a, lane);
+  const bool has_rows = first_row < it.n * p.group;
+
+  // LDS offsets of the operand reads: lane constants, tiles and pieces XORed or added in
+  const uint32_t k_off = (uint32_t)(mi * SH::kRB + ((kg ^ tree_swz_k<SH::kRB>(mi)) << 4));
+  uint32_t v_off;
+  if constexpr (SH::kQuant) {
+    const int r = mi >> 1;  // eight rows to sixteen lanes: tokens 4kg .. 4kg+3 and 16 + 4kg ..
+    const int row = r < 4 ? 4 * kg + r : 16 + 4 * kg + (r - 4);
+    v_off = (uint32_t)(SH::kArray + row * SH::kRB + (tree_swz_v<SH::kRB, true>(row) << 4) + (mi & 1) * 8);
+  } else {
+    const int row = 4 * kg + (mi >> 2);
+    v_off = (uint32_t)(SH::kArray + row * SH::kRB + ((((mi & 3) >> 1) ^ tree_swz_v<SH::kRB, false>(row)) << 4) + (mi & 1) * 8);
+  }
+
+  typedef TreeRows<SH, KV> Rows;
+  typedef typename Rows::OpK OpK;
+  typedef typename Rows::OpV OpV;
+
+  // Two row tiles over an 8-bit cache leave no registers for the operands' XORed offsets: there they are formed anew
+  // for every 32 tokens (an opaque copy of the first keeps the compiler from holding them through the loop).
+  auto fresh = [](uint32_t off) {
+    if (SH::kQuant && RTW > 1) asm volatile("" : "+v"(off));
+    return off;
+  };
+  // The operands of 32 tokens: K rows 16h + mi, elements of chunk c (16-bit), or chunks 2c and 2c + 1 (8-bit) ...
+  auto k_operand = [&](const uint8_t* tile, uint32_t ko, int c, int h) { return *(const u32x4*)(tile + (ko ^ (uint32_t)(c << 6)) + h * 16 * SH::kRB); };
+  // ... and V^T, head-dim tile dt.
+  auto v_operand = [&](const uint8_t* tile, uint32_t vo, int dt) {
+    if constexpr (SH::kQuant) {
+      typedef __attribute__((ext_vector_type(2))) int i32x2;
+      const i32x2 raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+          (__attribute__((address_space(3))) i32x2*)(tile + (vo ^ (uint32_t)(dt << 4))));
+      return __builtin_bit_cast(OpV, tree_widen<KV, SH::kVF16>((uint32_t)raw[0], (uint32_t)raw[1]));
+    } else {
+      const uint32_t at = vo ^ (uint32_t)(dt << 5);
+      const s16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(tile + at));
+      const s16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(tile + at + 16 * SH::kRB));
+      return __builtin_bit_cast(OpV, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  };
+  // S^T of N row tiles from `a` on over 32 tokens: every K operand serves all of them.
+  auto scores = [&](const uint8_t* tile, auto count, int a, f32x4 (&s)[decltype(count)::value][2]) {
+    constexpr int N = decltype(count)::value;
+    const uint32_t ko = fresh(k_off);
+#pragma unroll
+    for (int n = 0; n < N; ++n) s[n][0] = s[n][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < (SH::kQuant ? SH::kChunks / 2 : SH::kChunks); ++c) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const u32x4 raw = k_operand(tile, ko, c, h);
+        if constexpr (SH::kQuant) {
+          const OpK f0 = __builtin_bit_cast(OpK, tree_widen<KV, SH::kKF16>(raw[0], raw[1]));
+          const OpK f1 = __builtin_bit_cast(OpK, tree_widen<KV, SH::kKF16>(raw[2], raw[3]));
+#pragma unroll
+          for (int n = 0; n < N; ++n) {
+            s[n][h] = MmaOps<SH::kKF16>::run(f0, rows[a + n].qf[2 * c], s[n][h]);
+            s[n][h] = MmaOps<SH::kKF16>::run(f1, rows[a + n].qf[2 * c + 1], s[n][h]);
+          }
+        } else {
+          const OpK f = __builtin_bit_cast(OpK, raw);
+#pragma unroll
+          for (int n = 0; n < N; ++n) s[n][h] = MmaOps<SH::kKF16>::run(f, rows[a + n].qf[c], s[n][h]);
+        }
+      }
+    }
+  };
+  // One of the three per-token factors of 32 tokens (8-bit caches): 0 kscl, 1 lv, 2 rvs.
+  auto factor = [&](const uint8_t* stage, int piece, int which, f32x4 (&f)[2]) {
+    if constexpr (SH::kQuant) {
+      const float* src = (const float*)(stage + SH::kFactors) + which * SH::kTT + piece + 4 * kg;
+      f[0] = *(const f32x4*)src;
+      f[1] = *(const f32x4*)(src + 16);
+    }
+  };
+
+  // 32 tokens that every row sees.
+  auto attend = [&](const uint8_t* stage, int piece) {
+    const uint8_t* tile = stage + piece * SH::kRB;
+    f32x4 s[RTW][2];
+    scores(tile, std::integral_constant<int, RTW>{}, 0, s);
+    float x[RTW][8];
+    {
+      f32x4 kscl[2], lv[2];
+      factor(stage, piece, 0, kscl);
+      factor(stage, piece, 1, lv);
+#pragma unroll
+      for (int a = 0; a < RTW; ++a) rows[a].template scaled<false>(s[a], kscl, lv, p.scale_log2, 0, kg, x[a]);
+    }
+    // (the factors live as briefly as they can: two row tiles leave no register to spare)
+    if (SH::kQuant && RTW > 1) __builtin_amdgcn_sched_barrier(0);
+    f32x4 rvs[2];
+    factor(stage, piece, 2, rvs);
+    OpV pf[RTW];
+    float alpha[RTW];
+    bool moved = false;
+#pragma unroll
+    for (int a = 0; a < RTW; ++a) {
+      moved |= rows[a].template weights<false>(x[a], rvs, p.scale_log2, 0, kg, alpha[a]);
+      pf[a] = Rows::pack(x[a]);
+    }
+    if (moved) {
+#pragma unroll
+      for (int a = 0; a < RTW; ++a) {
+#pragma unroll
+        for (int dt = 0; dt < SH::kDT; ++dt) rows[a].acc[dt] *= alpha[a];
+      }
+    }
+    const uint32_t vo = fresh(v_off);
+#pragma unroll
+    for (int dt = 0; dt < SH::kDT; ++dt) {
+      const OpV vf = v_operand(tile, vo, dt);
+#pragma unroll
+      for (int a = 0; a < RTW; ++a) rows[a].acc[dt] = MmaOps<SH::kVF16>::run(vf, pf[a], rows[a].acc[dt]);
+    }
+  };
+
+  TreeRowMask masks[RTW];
+  // 32 tokens under the rows' bits, one row tile after the other.  `exact`: token by token (see the head of the file).
+  auto attend_masked = [&](const uint8_t* stage, int tb, int piece, bool exact) {
+    const uint8_t* tile = stage + piece * SH::kRB;
+#pragma unroll
+    for (int a = 0; a < RTW; ++a) {
+      f32x4 s[1][2];
+      scores(tile, std::integral_constant<int, 1>{}, a, s);
+      const uint32_t vis = masks[a].bits(it, tb + piece);
+      float w[8], alpha;
+      {
+        f32x4 kscl[2], lv[2];
+        factor(stage, piece, 0, kscl);
+        factor(stage, piece, 1, lv);
+        rows[a].template scaled<true>(s[0], kscl, lv, p.scale_log2, vis, kg, w);
+      }
+      f32x4 rvs[2];
+      factor(stage, piece, 2, rvs);
+      if (rows[a].template weights<true>(w, rvs, p.scale_log2, vis, kg, alpha)) {
+#pragma unroll
+        for (int dt = 0; dt < SH::kDT; ++dt) rows[a].acc[dt] *= alpha;
+      }
+      if (KV != XLLM_HIP_INT8 && exact) {
+#pragma unroll
+        for (int dt = 0; dt < SH::kDT; ++dt) {
+          f32x4 o = rows[a].acc[dt];
+#pragma unroll 1
+          for (int t = 0; t < 32; ++t) {
+            // the weight of token t lies with lane kg' = (t >> 2) & 3 of the row's four, as its number 4 (t >> 4) + (t & 3)
+            const int idx = 4 * (t >> 4) + (t & 3);
+            float mine = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mine = idx == i ? w[i] : mine;
+            const float wt = __shfl(mine, ((t >> 2) & 3) * 16 + mi);
+            const int row = piece + t, at = (dt * 16 + 4 * kg) * SH::kEB;
+            const uint8_t* v = stage + SH::kArray + row * SH::kRB + (((at >> 4) ^ tree_swz_v<SH::kRB, SH::kQuant>(row)) << 4) + (at & 15);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (vis >> t) & 1 ? __builtin_fmaf(wt, Elem<KV>::load(v, e), o[e]) : o[e];
+          }
+          rows[a].acc[dt] = o;
+        }
+      } else {
+        const OpV pf = Rows::pack(w);
+        const uint32_t vo = fresh(v_off);
+#pragma unroll
+        for (int dt = 0; dt < SH::kDT; ++dt) rows[a].acc[dt] = MmaOps<SH::kVF16>::run(v_operand(tile, vo, dt), pf, rows[a].acc[dt]);
+      }
+    }
+  };
+
+  // Tile i from `here`: its loads have landed (every wave waits for its own), the waves meet — nobody reads `next` any
+  // more — tile i + 1 goes in flight into `next`, tile i is attended.  The two stages are LDS arrays of their own and
+  // the loop over tiles that every row sees is written out for both, so that the compiler can tell the loads in
+  // flight from the tile being read and does not wait for them.
+  auto step = [&](int i, uint8_t* here, uint8_t* next) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    ld.factors(p, here);
+    __syncthreads();
+    if (i + 1 < iters) ld.issue(p, it, t0 + (i + 1) * SH::kTT, next);
+    if (!has_rows) return;
+#pragma unroll 1
+    for (int piece = 32 * tg; piece < SH::kTT; piece += 32 * TS) attend(here, piece);
+  };
+  // Tiles whose tokens all lie in the context, and within the length.
+  const int whole = it.prefix > t0 ? min((it.prefix - t0) / SH::kTT, iters) : 0;
+  int i = 0;
+  for (; i + 2 <= whole; i += 2) {
+    step(i, stage0, stage1);
+    step(i + 1, stage1, stage0);
+  }
+  // The rest: an odd tile of the context, the last of the context with the drafted tokens behind it, and so on.  (The
+  // masks are fetched only here: two row tiles have no registers for them in the loop above.)
+  if (i < iters) {
+#pragma unroll
+    for (int a = 0; a < RTW; ++a) masks[a].init(p, it, first_row + 16 * a, lane);
+  }
+  for (; i < iters; ++i) {
+    uint8_t* here = (i & 1) != 0 ? stage1 : stage0;
+    const int tb = t0 + i * SH::kTT;
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    ld.factors(p, here);
+    if (KV != XLLM_HIP_INT8) {
+      const bool bad = ld.look_through(tb, it.len, here);
+      if (lane == 0) found[i & 1][wave] = bad;
+    }
+    __syncthreads();  // (factors, zeros and findings are in LDS too)
+    if (i + 1 < iters) ld.issue(p, it, tb + SH::kTT, (i & 1) != 0 ? stage0 : stage1);
+    if (!has_rows) continue;
+    bool exact = false;
+    if (KV != XLLM_HIP_INT8) {
+      const int* f = found[i & 1];
+      exact = __builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3]) != 0;
+    }
+#pragma unroll 1
+    for (int piece = 32 * tg; piece < SH::kTT && tb + piece < it.t_end; piece += 32 * TS) attend_masked(here, tb, piece, exact);
+  }
+
+  // End of the item.
+  const float neg_inf = -INFINITY;
+  if constexpr (TS == 2) {
+    // the second wave of a row tile hands over its sums; nothing is in flight any more
+    __syncthreads();
+    uint8_t* xch = (wave & 1) != 0 ? stage1 : stage0;
+    Rows& r = rows[0];
+    if (tg == 1) {
+      *(float*)(xch + lane * 4) = r.m_run;
+      *(float*)(xch + 256 + lane * 4) = r.l_run;
+#pragma unroll
+      for (int dt = 0; dt < SH::kDT; ++dt) *(f32x4*)(xch + 512 + dt * 1024 + lane * 16) = r.acc[dt];
+    }
+    __syncthreads();
+    if (tg == 1) return;
+    const float m2 = *(const float*)(xch + lane * 4), l2 = *(const float*)(xch + 256 + lane * 4);
+    const float m = fmaxf(r.m_run, m2);
+    const float m_safe = m == neg_inf ? 0.0f : m;
+    const float a1 = __builtin_amdgcn_exp2f(r.m_run - m_safe), a2 = __builtin_amdgcn_exp2f(m2 - m_safe);
+    r.m_run = m;
+    r.l_run = r.l_run * a1 + l2 * a2;
+#pragma unroll
+    for (int dt = 0; dt < SH::kDT; ++dt) {
+      const f32x4 o = *(const f32x4*)(xch + 512 + dt * 1024 + lane * 16);
+      r.acc[dt] = r.acc[dt] * a1 + o * a2;
+    }
+  }
+  if (!has_rows) return;
+#pragma unroll
+  for (int a = 0; a < RTW; ++a) {
+    Rows& r = rows[a];
+    const float l = kg_sum(r.l_run);
+    const int row = tree_row(p, it, first_row + 16 * a, lane);
+    if (row < 0) continue;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a NaN stays one)
+    const float lse2 = l == 0.0f ? neg_inf : r.m_run + __builtin_amdgcn_logf(l);
+    const int j = row / p.group;
+    const int head = it.hk * p.group + (row - j * p.group);
+    const int64_t token = it.q0 + j;
+    if (it.chunks == 1) {
+      if (kg == 0 && p.lse != nullptr) p.lse[token * p.num_q_heads + head] = lse2;
+      uint16_t* out = (uint16_t*)p.out + token * p.out_token_stride + (int64_t)head * D + 4 * kg;
+#pragma unroll
+      for (int dt = 0; dt < SH::kDT; ++dt) {
+        const f32x4 o = r.acc[dt] * inv;
+        typedef MmaOps<SH::kQF16> M;
+        *(u32x2*)(out + dt * 16) = u32x2{M::pack(o[0], o[1]), M::pack(o[2], o[3])};
+      }
+    } else {
+      const int64_t prow = ((int64_t)it.b * p.slots + it.chunk) * ((int64_t)p.n * p.num_q_heads) + (int64_t)j * p.num_q_heads + head;
+      if (kg == 0) p.partial_lse[prow] = lse2;
+      float* out = p.partial_out + prow * D + 4 * kg;
+#pragma unroll
+      for (int dt = 0; dt < SH::kDT; ++dt) *(f32x4*)(out + dt * 16) = r.acc[dt] * inv;
+    }
+  }
+}
+
+}  // namespace xllm_hip
