@@ -23,13 +23,15 @@ constexpr int kTreeMaxWords = 8;
 constexpr int kTreeMaxSlots = 64;    // chunks per sequence: a lane each in the merge
 constexpr int kTreeMinChunk = 256;   // tokens: a shorter chunk costs more in its partial than it saves
 
-// Chunks a sequence may have: enough that the launch has 2048 items, no more than the merge holds, and no more than
-// 64 MiB of partials.  Sizes only, so that one workspace serves every step of these sizes.
+// Chunks a sequence may have: enough that the launch has 2048 items (and four, for lengths that differ), no more than
+// the merge holds, and no more than 512 MiB of partials.  Sizes only, so that one workspace serves every step of these
+// sizes.
 static int tree_slots(int64_t batch, int64_t n, int64_t hq, int64_t hkv, int64_t d) {
   const int64_t items = batch * hkv;
   int64_t s = items > 0 ? (2048 + items - 1) / items : 1;
+  s = s > 4 ? s : 4;
   const int64_t row_bytes = batch * n * hq * (d + 1) * 4;
-  const int64_t fit = row_bytes > 0 ? ((int64_t)64 << 20) / row_bytes : kTreeMaxSlots;
+  const int64_t fit = row_bytes > 0 ? ((int64_t)512 << 20) / row_bytes : kTreeMaxSlots;
   s = s < fit ? s : fit;
   s = s < kTreeMaxSlots ? s : kTreeMaxSlots;
   return s > 1 ? (int)s : 1;
@@ -96,11 +98,12 @@ static TreeForm tree_form(const xllm_hip_kv_cache* c, const xllm_hip_decode_args
 // chunks as the workspace holds, of at least kTreeMinChunk tokens.  With them, the cut whose step is predicted to end
 // first, counted in tokens a workgroup gets through (`at_once` of them run together):
 //   nearly equal lengths   rounds of equal items:  ceil(items / at_once) * (chunk + kItemTokens)
-//   ragged lengths         items / at_once * (mean chunk + kItemTokens), and half a chunk until the last one ends
+//   ragged lengths         the longest chunk while all items run together; else the items' tokens over `at_once`, and
+//                          half a chunk until the last one ends
 // plus, where sequences are cut, the merge's launch and the partial results, written once and read once (a row's 4
 // bytes per element against the 2 * eb a cached token takes, shared by the whole GPU).
 static void choose_chunks(const xllm_hip_decode_args* a, const TreeForm& form, int eb, TreeParams& p) {
-  constexpr int64_t kItemTokens = 64;
+  constexpr int64_t kItemTokens = 128;
   constexpr int64_t kMergeTokens = 128;
   auto whole = [&](int64_t tokens) { return (tokens + p.tile - 1) / p.tile * p.tile; };
   const int64_t longest = a->max_seq_len;
@@ -126,11 +129,12 @@ static void choose_chunks(const xllm_hip_decode_args* a, const TreeForm& form, i
     if (equal) {
       const int64_t items = lanes * p.batch * ((longest + chunk - 1) / chunk);
       t = (double)((items + form.slots - 1) / form.slots) * (double)(chunk + kItemTokens);
-      if (cut > 1) t += (double)items * item_rows * 4.0 / eb / form.slots;
+      if (cut > 1) t += (double)items * item_rows * 2.0 / eb / form.slots;
     } else {
       const double items = (double)lanes * ((double)total / (double)chunk + 0.5 * p.batch);
-      t = ((double)lanes * (double)total + items * kItemTokens) / form.slots + 0.5 * (double)chunk;
-      if (cut > 1) t += items * item_rows * 4.0 / eb / form.slots;
+      t = items <= (double)form.slots ? (double)(chunk + kItemTokens)
+                                      : ((double)lanes * (double)total + items * kItemTokens) / form.slots + 0.5 * (double)chunk;
+      if (cut > 1) t += items * item_rows * 2.0 / eb / form.slots;
     }
     if (cut > 1) t += kMergeTokens;
     if (best_cut == 0 || t < best) {
@@ -140,6 +144,18 @@ static void choose_chunks(const xllm_hip_decode_args* a, const TreeForm& form, i
   }
   p.chunk = (int32_t)whole((longest + best_cut - 1) / best_cut);
   p.slots = best_cut;
+}
+
+template <int Q_DT>
+static void launch_tree_merge(const TreeParams& p, hipStream_t st) {
+  const dim3 grid((unsigned)((p.n * p.num_q_heads + 15) / 16), (unsigned)p.batch);
+  if (p.head_dim <= 64) {
+    tree_merge_kernel<Q_DT, 16><<<grid, 256, 0, st>>>(p);
+  } else if (p.head_dim <= 128) {
+    tree_merge_kernel<Q_DT, 32><<<grid, 256, 0, st>>>(p);
+  } else {
+    tree_merge_kernel<Q_DT, 64><<<grid, 256, 0, st>>>(p);
+  }
 }
 
 template <int QT, int KV, int D>
@@ -221,6 +237,7 @@ extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
   if (mask_words > kTreeMaxWords) {
     return fail(XLLM_HIP_UNSUPPORTED, "mask_words %d is larger than %d", mask_words, kTreeMaxWords);
   }
+  if (a->batch > 65535) return fail(XLLM_HIP_UNSUPPORTED, "batch %d is larger than 65535", a->batch);
   XLLM_HIP_REQUIRE(a->max_seq_len >= 0 && a->total_kv_len >= 0, "max_seq_len or total_kv_len is negative");
   if (a->batch == 0) return XLLM_HIP_OK;
   XLLM_HIP_REQUIRE(a->q != nullptr && a->out != nullptr && tree_mask != nullptr, "q, out or tree_mask is NULL");
@@ -314,13 +331,12 @@ extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
   }
   int rc = check_launch("tree attention kernel");
   if (rc != XLLM_HIP_OK || p.slots == 1) return rc;
-  const unsigned merge_grid = (unsigned)(((int64_t)p.batch * p.n * p.num_q_heads + 3) / 4);
   if (p.q_dtype == XLLM_HIP_BF16) {
-    tree_merge_kernel<XLLM_HIP_BF16><<<merge_grid, 256, 0, st>>>(p);
+    launch_tree_merge<XLLM_HIP_BF16>(p, st);
   } else if (p.q_dtype == XLLM_HIP_FP16) {
-    tree_merge_kernel<XLLM_HIP_FP16><<<merge_grid, 256, 0, st>>>(p);
+    launch_tree_merge<XLLM_HIP_FP16>(p, st);
   } else {
-    tree_merge_kernel<XLLM_HIP_FP32><<<merge_grid, 256, 0, st>>>(p);
+    launch_tree_merge<XLLM_HIP_FP32>(p, st);
   }
   return check_launch("tree_merge_kernel");
 }

@@ -91,53 +91,100 @@ __global__ void __launch_bounds__(64) tree_generic_kernel(TreeParams p) {
   }
 }
 
-// Rows of cut sequences: out = sum_c 2^(lse_c - lse) partial_c, lse = log2 sum_c 2^lse_c.  One wave per row, four rows
-// to a workgroup; a chunk that saw nothing has lse -inf, weight 0 and a partial of zeros.
-template <int Q_DT>
+// Rows of cut sequences: out = sum_c 2^(lse_c - lse) partial_c, lse = log2 sum_c 2^lse_c; a chunk that saw nothing has
+// lse -inf, weight 0 and a partial of zeros.  Bound by the partials' bytes and by the latency of their loads, so four
+// floats to a lane, D / 4 lanes to a chunk's row (a wave has 64 / (D / 4) chunks' rows at a time), and four query rows
+// to a wave, whose loads all go out before the first is used.
+template <int Q_DT, int COLS>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
+  static_assert(COLS == 16 || COLS == 32 || COLS == 64, "lanes that share a chunk's row, four columns each");
+  constexpr int kAtOnce = 64 / COLS;
+  constexpr int kUnroll = COLS == 64 ? 4 : 2;  // loads per query row in flight
+  constexpr int kRows = 4;
   const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t per_seq = (int64_t)p.n * p.num_q_heads;
-  const int64_t b64 = unit / per_seq;
-  if (b64 >= p.batch) return;
-  const int b = (int)b64;
-  const int rem = (int)(unit - b64 * per_seq);
-  const int j = rem / p.num_q_heads;
-  const int head = rem - j * p.num_q_heads;
+  // (grid: rows of a sequence, sequences; the workgroups of a sequence that was not cut end here)
+  const int b = blockIdx.y;
+  const int chunks = tree_chunks(p, tree_kv_length(p, b));
+  if (chunks == 1) return;  // written by the attention kernel
+  const int per_seq = p.n * p.num_q_heads;
   int64_t q0;
   int count;
   tree_rows(p, b, q0, count);
-  if (j >= count) return;
-  const int chunks = tree_chunks(p, tree_kv_length(p, b));
-  if (chunks == 1) return;  // written by the attention kernel
+  const int rows = (count < p.n ? count : p.n) * p.num_q_heads;
+  const int r0 = ((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6)) * kRows;
+  if (r0 >= rows) return;
   const int D = p.head_dim;
   const float neg_inf = -INFINITY;
-  const int64_t first = (int64_t)b * p.slots * per_seq + rem;  // chunk c: + c * per_seq
-  // slots <= 64: a chunk to a lane
-  const float l = lane < chunks ? p.partial_lse[first + lane * per_seq] : neg_inf;
-  const float m = wave_max(l);
-  const float m_safe = m == neg_inf ? 0.0f : m;
-  const float e = __builtin_amdgcn_exp2f(l - m_safe);
-  const float total = wave_sum(e);
-  float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int c = 0; c < chunks; ++c) {
-    const float w = __shfl(e, c);
-    const float* src = p.partial_out + (first + c * per_seq) * D;
+  const int64_t first = (int64_t)b * p.slots * per_seq;  // row r of chunk c: + c * per_seq + r
+  const int col = (lane % COLS) * 4;
+  const int mine = lane / COLS;
+  const bool vec = (D & 3) == 0;
+  f32x4 v[kRows][kUnroll];
+  float l[kRows];
+  auto load = [&](int c0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 64 * i;
-      if (d < D) o[i] += w * src[d];
+    for (int k = 0; k < kRows; ++k) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int c = c0 + u * kAtOnce + mine;
+        v[k][u] = f32x4{0, 0, 0, 0};
+        if (c < chunks && col < D && r0 + k < rows) {
+          const float* src = p.partial_out + (first + (int64_t)c * per_seq + r0 + k) * D + col;
+          if (vec) {
+            v[k][u] = *(const f32x4*)src;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[k][u][e] = col + e < D ? src[e] : 0.0f;
+          }
+        }
+      }
+    }
+  };
+  // slots <= 64: a chunk to a lane
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    l[k] = lane < chunks && r0 + k < rows ? p.partial_lse[first + (int64_t)lane * per_seq + r0 + k] : neg_inf;
+  }
+  load(0);  // (on their way while the weights are formed)
+  float e[kRows], m[kRows], total[kRows];
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    m[k] = wave_max(l[k]);
+    e[k] = __builtin_amdgcn_exp2f(l[k] - (m[k] == neg_inf ? 0.0f : m[k]));
+    total[k] = wave_sum(e[k]);
+  }
+  f32x4 o[kRows];
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) o[k] = f32x4{0, 0, 0, 0};
+  for (int c0 = 0; c0 < chunks; c0 += kAtOnce * kUnroll) {
+    if (c0 > 0) load(c0);
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) o[k] += __shfl(e[k], (c0 + u * kAtOnce + mine) & 63) * v[k][u];
     }
   }
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  const int64_t row = q0 + j;
-  if (lane == 0 && p.lse != nullptr) {
-    p.lse[row * p.num_q_heads + head] = total == 0.0f ? neg_inf : m + __builtin_amdgcn_logf(total);
-  }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 64 * i;
-    if (d < D) Elem<Q_DT>::store(p.out, row * p.out_token_stride + (int64_t)head * D + d, o[i] * inv);
+  for (int k = 0; k < kRows; ++k) {
+    if (r0 + k >= rows) break;
+#pragma unroll
+    for (int s = COLS; s < 64; s <<= 1) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o[k][x] += __shfl_xor(o[k][x], s);
+    }
+    const float inv = total[k] == 0.0f ? 0.0f : 1.0f / total[k];
+    const int j = (r0 + k) / p.num_q_heads;
+    const int head = r0 + k - j * p.num_q_heads;
+    const int64_t row = q0 + j;
+    if (lane == 0 && p.lse != nullptr) {
+      p.lse[row * p.num_q_heads + head] = total[k] == 0.0f ? neg_inf : m[k] + __builtin_amdgcn_logf(total[k]);
+    }
+    if (mine == 0) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (col + x < D) Elem<Q_DT>::store(p.out, row * p.out_token_stride + (int64_t)head * D + col + x, o[k][x] * inv);
+      }
+    }
   }
 }
 

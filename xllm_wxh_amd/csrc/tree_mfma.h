@@ -113,7 +113,14 @@ __device__ inline bool tree_not_finite(u32x4 v) {
 // One wave's share of the loads: where its rows lie, and the loads of a tile.
 template <class SH, int KV>
 struct TreeLoader {
-  uint32_t off_k[SH::kLoads], off_v[SH::kLoads];  // byte offset of this lane's piece from the first of the 16 tokens
+  // Byte offset of this lane's piece from the first row of a load instruction.  The rows of further instructions differ
+  // in the swizzle by few bits, so few of these are distinct: K's in the row's low three bits (kVarK instructions in
+  // turn), V's in the low two, or over an 8-bit cache in the group of 16.
+  static constexpr int kGroups = SH::kRW / 16;
+  static constexpr int kPer = SH::kLoads / kGroups;  // load instructions per group of 16 tokens
+  static constexpr int kVarK = SH::kRPI >= 8 ? 1 : 8 / SH::kRPI;
+  static constexpr int kVarV = SH::kQuant ? kGroups : SH::kRPI >= 4 ? 1 : 4 / SH::kRPI;
+  uint32_t off_k[kVarK], off_v[kVarV];
   int wave, lane;
   float sc;  // the scale in flight: lanes 0..31 the K scales of the wave's tokens, 32..63 the V scales
   uint32_t sc_off;
@@ -121,14 +128,13 @@ struct TreeLoader {
   __device__ inline void init(const TreeParams& p, int w, int l) {
     wave = w;
     lane = l;
-    const int pos = l % SH::kPPR;
+    const int pos = l % SH::kPPR, lr = l / SH::kPPR;
+    const uint32_t at = (uint32_t)(lr * p.stride_slot) * SH::kEB;
 #pragma unroll
-    for (int q = 0; q < SH::kLoads; ++q) {
-      const int rw = q * SH::kRPI + l / SH::kPPR;  // row among the wave's
-      const int row = w * SH::kRW + rw;            // row of the tile
-      const uint32_t at = (uint32_t)((rw & 15) * p.stride_slot) * SH::kEB;
-      off_k[q] = at + ((pos ^ tree_swz_k<SH::kRB>(row)) << 4);
-      off_v[q] = at + ((pos ^ tree_swz_v<SH::kRB, SH::kQuant>(row)) << 4);
+    for (int v = 0; v < kVarK; ++v) off_k[v] = at + ((pos ^ tree_swz_k<SH::kRB>(w * SH::kRW + v * SH::kRPI + lr)) << 4);
+#pragma unroll
+    for (int v = 0; v < kVarV; ++v) {
+      off_v[v] = at + ((pos ^ tree_swz_v<SH::kRB, SH::kQuant>(w * SH::kRW + v * (SH::kQuant ? 16 : SH::kRPI) + lr)) << 4);
     }
     sc = 0.0f;
     sc_off = 0;
@@ -144,8 +150,6 @@ struct TreeLoader {
   }
 
   __device__ inline void issue(const TreeParams& p, const TreeItem& it, int tb, uint8_t* stage) {
-    constexpr int kGroups = SH::kRW / 16;
-    constexpr int kPer = SH::kLoads / kGroups;  // load instructions per group
     const int first = tb + wave * SH::kRW;
     uint8_t* kl = stage + wave * (SH::kRW * SH::kRB);
     uint8_t* vl = kl + SH::kArray;
@@ -163,10 +167,13 @@ struct TreeLoader {
       }
       const uint8_t* kb = p.k_cache + elem * SH::kEB;
       const uint8_t* vb = p.v_cache + elem * SH::kEB;
+      const int64_t next = (int64_t)SH::kRPI * p.stride_slot * SH::kEB;  // from one instruction's rows to the next's
 #pragma unroll
-      for (int q = g * kPer; q < (g + 1) * kPer; ++q) XLLM_HIP_GLOBAL_TO_LDS_16(kb + off_k[q], kl + q * 1024);
+      for (int q = 0; q < kPer; ++q) XLLM_HIP_GLOBAL_TO_LDS_16(kb + q * next + off_k[q % kVarK], kl + (g * kPer + q) * 1024);
 #pragma unroll
-      for (int q = g * kPer; q < (g + 1) * kPer; ++q) XLLM_HIP_GLOBAL_TO_LDS_16(vb + off_v[q], vl + q * 1024);
+      for (int q = 0; q < kPer; ++q) {
+        XLLM_HIP_GLOBAL_TO_LDS_16(vb + q * next + off_v[SH::kQuant ? g : q % kVarV], vl + (g * kPer + q) * 1024);
+      }
     }
     if constexpr (SH::kQuant) {
       // lane = (array, token among the wave's, 16 of them twice where there are only 16)
@@ -198,9 +205,9 @@ struct TreeLoader {
     }
   }
 
-  // The wave's V rows of a masked tile, landed: zeros over the rows past the length; whether another holds something
-  // that is not finite.
-  __device__ inline bool look_through(int tb, int len, uint8_t* stage) const {
+  // The wave's V rows of a masked tile, landed: zeros over the rows past the length; whether a drafted token's holds
+  // something that is not finite.
+  __device__ inline bool look_through(int tb, int prefix, int len, uint8_t* stage) const {
     bool bad = false;
     if constexpr (KV != XLLM_HIP_INT8) {
 #pragma unroll
@@ -209,7 +216,7 @@ struct TreeLoader {
         u32x4* at = (u32x4*)(stage + SH::kArray + wave * (SH::kRW * SH::kRB) + q * 1024 + lane * 16);
         if (tok >= len) {
           *at = u32x4{0, 0, 0, 0};
-        } else {
+        } else if (tok >= prefix) {
           bad = bad || tree_not_finite<KV>(*at);
         }
       }
@@ -426,10 +433,10 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
   typedef typename Rows::OpK OpK;
   typedef typename Rows::OpV OpV;
 
-  // Two row tiles over an 8-bit cache leave no registers for the operands' XORed offsets: there they are formed anew
-  // for every 32 tokens (an opaque copy of the first keeps the compiler from holding them through the loop).
+  // Two row tiles, or head_dim 256, leave no registers for the operands' XORed offsets: there they are formed anew for
+  // every 32 tokens (an opaque copy of the first keeps the compiler from holding them through the loop).
   auto fresh = [](uint32_t off) {
-    if (SH::kQuant && RTW > 1) asm volatile("" : "+v"(off));
+    if (RTW > 1 || D == 256) asm volatile("" : "+v"(off));
     return off;
   };
   // The operands of 32 tokens: K rows 16h + mi, elements of chunk c (16-bit), or chunks 2c and 2c + 1 (8-bit) ...
@@ -484,18 +491,23 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
     }
   };
 
-  // 32 tokens that every row sees.
-  auto attend = [&](const uint8_t* stage, int piece) {
+  // 32 tokens: those every row sees, or (MASKED) under the rows' bits.
+  TreeRowMask masks[RTW];
+  auto attend = [&](const uint8_t* stage, int tb, int piece, auto masked) {
+    constexpr bool MASKED = decltype(masked)::value;
     const uint8_t* tile = stage + piece * SH::kRB;
     f32x4 s[RTW][2];
     scores(tile, std::integral_constant<int, RTW>{}, 0, s);
+    uint32_t vis[RTW];
+#pragma unroll
+    for (int a = 0; a < RTW; ++a) vis[a] = MASKED ? masks[a].bits(it, tb + piece) : 0u;
     float x[RTW][8];
     {
       f32x4 kscl[2], lv[2];
       factor(stage, piece, 0, kscl);
       factor(stage, piece, 1, lv);
 #pragma unroll
-      for (int a = 0; a < RTW; ++a) rows[a].template scaled<false>(s[a], kscl, lv, p.scale_log2, 0, kg, x[a]);
+      for (int a = 0; a < RTW; ++a) rows[a].template scaled<MASKED>(s[a], kscl, lv, p.scale_log2, vis[a], kg, x[a]);
     }
     // (the factors live as briefly as they can: two row tiles leave no register to spare)
     if (SH::kQuant && RTW > 1) __builtin_amdgcn_sched_barrier(0);
@@ -506,7 +518,7 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
     bool moved = false;
 #pragma unroll
     for (int a = 0; a < RTW; ++a) {
-      moved |= rows[a].template weights<false>(x[a], rvs, p.scale_log2, 0, kg, alpha[a]);
+      moved |= rows[a].template weights<MASKED>(x[a], rvs, p.scale_log2, vis[a], kg, alpha[a]);
       pf[a] = Rows::pack(x[a]);
     }
     if (moved) {
@@ -525,9 +537,9 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
     }
   };
 
-  TreeRowMask masks[RTW];
-  // 32 tokens under the rows' bits, one row tile after the other.  `exact`: token by token (see the head of the file).
-  auto attend_masked = [&](const uint8_t* stage, int tb, int piece, bool exact) {
+  // The same where V holds something that is not finite: token by token, each row under its own bits, a row tile after
+  // the other (see the head of the file).
+  auto attend_exact = [&](const uint8_t* stage, int tb, int piece) {
     const uint8_t* tile = stage + piece * SH::kRB;
 #pragma unroll
     for (int a = 0; a < RTW; ++a) {
@@ -547,30 +559,23 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
 #pragma unroll
         for (int dt = 0; dt < SH::kDT; ++dt) rows[a].acc[dt] *= alpha;
       }
-      if (KV != XLLM_HIP_INT8 && exact) {
 #pragma unroll
-        for (int dt = 0; dt < SH::kDT; ++dt) {
-          f32x4 o = rows[a].acc[dt];
+      for (int dt = 0; dt < SH::kDT; ++dt) {
+        f32x4 o = rows[a].acc[dt];
 #pragma unroll 1
-          for (int t = 0; t < 32; ++t) {
-            // the weight of token t lies with lane kg' = (t >> 2) & 3 of the row's four, as its number 4 (t >> 4) + (t & 3)
-            const int idx = 4 * (t >> 4) + (t & 3);
-            float mine = 0.0f;
+        for (int t = 0; t < 32; ++t) {
+          // the weight of token t lies with lane kg' = (t >> 2) & 3 of the row's four, as its number 4 (t >> 4) + (t & 3)
+          const int idx = 4 * (t >> 4) + (t & 3);
+          float mine = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) mine = idx == i ? w[i] : mine;
-            const float wt = __shfl(mine, ((t >> 2) & 3) * 16 + mi);
-            const int row = piece + t, at = (dt * 16 + 4 * kg) * SH::kEB;
-            const uint8_t* v = stage + SH::kArray + row * SH::kRB + (((at >> 4) ^ tree_swz_v<SH::kRB, SH::kQuant>(row)) << 4) + (at & 15);
+          for (int i = 0; i < 8; ++i) mine = idx == i ? w[i] : mine;
+          const float wt = __shfl(mine, ((t >> 2) & 3) * 16 + mi);
+          const int row = piece + t, at = (dt * 16 + 4 * kg) * SH::kEB;
+          const uint8_t* v = stage + SH::kArray + row * SH::kRB + (((at >> 4) ^ tree_swz_v<SH::kRB, SH::kQuant>(row)) << 4) + (at & 15);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = (vis >> t) & 1 ? __builtin_fmaf(wt, Elem<KV>::load(v, e), o[e]) : o[e];
-          }
-          rows[a].acc[dt] = o;
+          for (int e = 0; e < 4; ++e) o[e] = (vis >> t) & 1 ? __builtin_fmaf(wt, Elem<KV>::load(v, e), o[e]) : o[e];
         }
-      } else {
-        const OpV pf = Rows::pack(w);
-        const uint32_t vo = fresh(v_off);
-#pragma unroll
-        for (int dt = 0; dt < SH::kDT; ++dt) rows[a].acc[dt] = MmaOps<SH::kVF16>::run(v_operand(tile, vo, dt), pf, rows[a].acc[dt]);
+        rows[a].acc[dt] = o;
       }
     }
   };
@@ -586,7 +591,7 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
     if (i + 1 < iters) ld.issue(p, it, t0 + (i + 1) * SH::kTT, next);
     if (!has_rows) return;
 #pragma unroll 1
-    for (int piece = 32 * tg; piece < SH::kTT; piece += 32 * TS) attend(here, piece);
+    for (int piece = 32 * tg; piece < SH::kTT; piece += 32 * TS) attend(here, 0, piece, std::false_type{});
   };
   // Tiles whose tokens all lie in the context, and within the length.
   const int whole = it.prefix > t0 ? min((it.prefix - t0) / SH::kTT, iters) : 0;
@@ -606,20 +611,29 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
     const int tb = t0 + i * SH::kTT;
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     ld.factors(p, here);
-    if (KV != XLLM_HIP_INT8) {
-      const bool bad = ld.look_through(tb, it.len, here);
+    const bool masked = tb + SH::kTT > it.prefix;
+    if (KV != XLLM_HIP_INT8 && masked) {
+      const bool bad = ld.look_through(tb, it.prefix, it.len, here);
       if (lane == 0) found[i & 1][wave] = bad;
     }
     __syncthreads();  // (factors, zeros and findings are in LDS too)
     if (i + 1 < iters) ld.issue(p, it, tb + SH::kTT, (i & 1) != 0 ? stage0 : stage1);
     if (!has_rows) continue;
     bool exact = false;
-    if (KV != XLLM_HIP_INT8) {
+    if (KV != XLLM_HIP_INT8 && masked) {
       const int* f = found[i & 1];
       exact = __builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3]) != 0;
     }
 #pragma unroll 1
-    for (int piece = 32 * tg; piece < SH::kTT && tb + piece < it.t_end; piece += 32 * TS) attend_masked(here, tb, piece, exact);
+    for (int piece = 32 * tg; piece < SH::kTT && tb + piece < it.t_end; piece += 32 * TS) {
+      if (tb + piece + 32 <= it.prefix) {
+        attend(here, tb, piece, std::false_type{});
+      } else if (KV != XLLM_HIP_INT8 && exact) {
+        attend_exact(here, tb, piece);
+      } else {
+        attend(here, tb, piece, std::true_type{});
+      }
+    }
   }
 
   // End of the item.

@@ -103,16 +103,16 @@ __device__ inline void tree_rows(const TreeParams& p, int b, int64_t& q0, int& c
 
 constexpr int kTreeXcds = 8;  // workgroup x runs on XCD x % 8
 
-// Items in their natural order are (sequence, chunk slot, kv head, row group), row group fastest: the row groups of
-// one (chunk, kv head) read the same K and V.
+// Items in their natural order are (chunk slot, sequence, kv head, row group), row group fastest: the row groups of one
+// (chunk, kv head) read the same K and V, and the sequences' last chunks, which are the short ones, run last.
 __device__ inline bool tree_item(const TreeParams& p, int id, int rows_per_item, TreeItem& it) {
   it.rg = id % p.row_groups;
   int rest = id / p.row_groups;
   it.hk = rest % p.num_kv_heads;
   rest /= p.num_kv_heads;
-  it.chunk = rest % p.slots;
-  it.b = rest / p.slots;
-  if (it.b >= p.batch) return false;
+  it.b = rest % p.batch;
+  it.chunk = rest / p.batch;
+  if (it.chunk >= p.slots) return false;
   int count;
   tree_rows(p, it.b, it.q0, count);
   it.n = count < p.n ? count : p.n;

@@ -816,7 +816,6 @@ def mrope_kv_write(qkv, num_heads_q, num_heads_kv, head_dim, cos_sin_cache, posi
 
 
 _tree_workspaces = {}
-TREE_WORKSPACE_BYTES = (64 << 20) + 4096  # what any sizes need at most
 
 
 def tree_workspace_bytes(batch, q_per_seq, num_q_heads, num_kv_heads, head_dim):
@@ -824,16 +823,18 @@ def tree_workspace_bytes(batch, q_per_seq, num_q_heads, num_kv_heads, head_dim):
 
 
 def _tree_workspace(device, nbytes):
-    """Scratch of a tree-attention call: one buffer per (device, stream) for eager calls, and memory of the graph's own
-    pool for a call under capture, so that no two graphs, and no graph and no eager call, share one."""
+    """Scratch of a tree-attention call: one buffer per (device, stream) for eager calls, which grows to the largest
+    call's need, and memory of the graph's own pool for a call under capture, so that no two graphs, and no graph and
+    no eager call, share one.  (A buffer that is outgrown goes back to torch's allocator, which hands it out again in
+    the order of the stream.)"""
     if nbytes == 0:
         return None
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device, torch.cuda.current_stream(device).cuda_stream)
     ws = _tree_workspaces.get(key)
-    if ws is None:
-        ws = _tree_workspaces[key] = torch.empty(TREE_WORKSPACE_BYTES, dtype=torch.uint8, device=device)
+    if ws is None or ws.numel() < nbytes:
+        ws = _tree_workspaces[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
     return ws
 
 
