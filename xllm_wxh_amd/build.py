@@ -73,7 +73,7 @@ def build_library(verbose=True, save_temps=False, extra_flags=()):
 
 TORCH_SHIM_NAME = "_xllm_hip_torch.so"
 TORCH_SHIM_PATH = os.path.join(PKG_DIR, TORCH_SHIM_NAME)
-TORCH_SHIM_SOURCES = ["ops_api.cpp", "attention.cpp", "pybind.cpp"]
+TORCH_SHIM_SOURCES = ["ops_api.cpp", "attention.cpp", "tree_step.cpp", "pybind.cpp"]
 
 
 def build_torch_shim(verbose=True):

@@ -5,6 +5,7 @@
 
 #include "attention.h"
 #include "ops_api.h"
+#include "tree_step.h"
 
 namespace py = pybind11;
 using xllm::KVCache;
@@ -186,4 +187,20 @@ PYBIND11_MODULE(_xllm_hip_torch, m) {
                                torch::Tensor cos_sin_cache, bool is_neox) {
     xllm::kernel::hip::rotary_embedding(positions, query, key, cos_sin_cache, is_neox);
   });
+
+  // The operators of a tree-speculative step; ops.py documents them and names their arguments.  Their errors become
+  // the package's own exception, with the C ABI's status.
+  py::register_exception_translator([](std::exception_ptr e) {
+    try {
+      if (e) std::rethrow_exception(e);
+    } catch (const xllm::kernel::hip::StatusError& x) {
+      const py::object type = py::module_::import("xllm_wxh_amd._lib").attr("XllmHipError");
+      PyErr_SetObject(type.ptr(), type(x.status(), x.what_without_backtrace()).ptr());
+    }
+  });
+  m.def("build_step_indices", &xllm::kernel::hip::build_step_indices);
+  m.def("tree_masks", &xllm::kernel::hip::tree_masks);
+  m.def("mrope_kv_write", &xllm::kernel::hip::mrope_kv_write);
+  m.def("batch_tree_decode", &xllm::kernel::hip::batch_tree_decode);
+  m.def("move_accepted_tokens", &xllm::kernel::hip::move_accepted_tokens);
 }

@@ -563,8 +563,13 @@ def dequant_from_paged_cache(key, value, key_cache, value_cache, key_cache_quant
                        context_lengths, max_context_len, context_seq_offset, block_tables, None, quant_mode, kv_layout)
 
 
-def _rope_args(qkv, num_q, num_k, num_v, head_dim, eps, q_weight, k_weight, cos_sin_cache, interleaved, positions,
-               round_each_op):
+def _rope_call(qkv, num_q, num_k, num_v, head_dim, eps, q_weight, k_weight, cos_sin_cache, interleaved, positions,
+               round_each_op, cache_desc=None, slot_mapping=None):
+    lib = _lib.load()
+    _require(qkv.is_cuda and qkv.dim() == 2 and qkv.stride(1) == 1, "qkv must be a 2-D GPU tensor, rows contiguous")
+    _require(positions.dtype in (torch.int64, torch.int32) and positions.dim() == 1 and positions.is_contiguous(),
+             "position_ids must be a contiguous 1-D int64 or int32 tensor")
+    _require(positions.numel() == qkv.size(0), "one position per token")
     _require(cos_sin_cache.dim() == 2 and cos_sin_cache.is_contiguous(), "cos_sin_cache must be [max_position, rotary_dim]")
     a = _lib.RopeArgs()
     a.qkv, a.token_stride, a.num_tokens = qkv.data_ptr(), qkv.stride(0), qkv.size(0)
@@ -582,18 +587,6 @@ def _rope_args(qkv, num_q, num_k, num_v, head_dim, eps, q_weight, k_weight, cos_
     a.positions = positions.data_ptr()
     a.positions_int32 = int(positions.dtype == torch.int32)
     a.interleave, a.round_each_op = int(bool(interleaved)), int(bool(round_each_op))
-    return a
-
-
-def _rope_call(qkv, num_q, num_k, num_v, head_dim, eps, q_weight, k_weight, cos_sin_cache, interleaved, positions,
-               round_each_op, cache_desc=None, slot_mapping=None):
-    lib = _lib.load()
-    _require(qkv.is_cuda and qkv.dim() == 2 and qkv.stride(1) == 1, "qkv must be a 2-D GPU tensor, rows contiguous")
-    _require(positions.dtype in (torch.int64, torch.int32) and positions.dim() == 1 and positions.is_contiguous(),
-             "position_ids must be a contiguous 1-D int64 or int32 tensor")
-    _require(positions.numel() == qkv.size(0), "one position per token")
-    a = _rope_args(qkv, num_q, num_k, num_v, head_dim, eps, q_weight, k_weight, cos_sin_cache, interleaved, positions,
-                   round_each_op)
     _lib.check(lib.xllm_hip_rope_kv_write(ctypes.byref(a), ctypes.byref(cache_desc) if cache_desc is not None else None,
                                           _ptr(slot_mapping), _stream()))
 
@@ -637,34 +630,23 @@ def rope_kv_write(qkv, num_heads_q, num_heads_kv, head_dim, cos_sin_cache, posit
 # a speculative step over a tree of drafted tokens
 # ---------------------------------------------------------------------------------------
 
-class _on_device:
-    """The tensors' device made current for a launch (nothing where it is already)."""
-
-    def __init__(self, device):
-        self.guard = None if device.index is None or device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+_shim_module = None
 
 
-def _on_gpu(first, *rest):
-    """Every tensor (None: absent) lives on the one GPU `first` lives on."""
-    _require(first.is_cuda, "the tensors must live on the GPU")
-    dev = first.device
-    for t in rest:
-        _require(t is None or t.device == dev, "the tensors must live on one GPU")
-    return dev
+def _shim():
+    """The libtorch host side: checks and launches of the operators below (a Python binding of the C ABI costs a
+    launch-bound call several times its kernel's time)."""
+    global _shim_module
+    if _shim_module is None:
+        _lib.load()
+        from . import _xllm_hip_torch
+        _shim_module = _xllm_hip_torch
+    return _shim_module
 
 
-def _vec32(t, n, name):
-    _require(t.dtype == torch.int32 and t.dim() == 1 and t.numel() == n and t.is_contiguous(),
-             "%s must be a contiguous int32 vector of %d entries" % (name, n))
+def _nhd(kv_layout):
+    _require(kv_layout in ("HND", "NHD"), "kv_layout must be 'HND' or 'NHD'")
+    return kv_layout == "NHD"
 
 
 def build_step_indices(cached_lens, block_pool, block_size, block_table, seq_lens, q_indptr, slot_mapping, positions, *,
@@ -682,63 +664,9 @@ def build_step_indices(cached_lens, block_pool, block_size, block_table, seq_len
     blocks are taken off the free list, in the order of the sequences, and appended to the rows of block_pool;
     held_blocks_out [batch] and free_head_out [2] (the new head; blocks that could not be had) receive the new state
     and must not be the old state's tensors.  All index tensors are int32 but positions."""
-    batch = cached_lens.numel()
-    _vec32(cached_lens, batch, "cached_lens")
-    _vec32(seq_lens, batch, "seq_lens")
-    _vec32(q_indptr, batch + 1, "q_indptr")
-    for name, t in (("new_lens", new_lens), ("request_ids", request_ids), ("held_blocks", held_blocks),
-                    ("held_blocks_out", held_blocks_out), ("paged_kv_last_page_len", paged_kv_last_page_len)):
-        if t is not None:
-            _vec32(t, batch, name)
-    for name, t in (("block_pool", block_pool), ("block_table", block_table)):
-        _require(t.dtype == torch.int32 and t.dim() == 2 and t.size(1) >= 1 and t.stride(1) == 1,
-                 "%s must be int32 [rows, width], rows contiguous" % name)
-    _require(block_pool.size(0) >= 1, "block_pool holds no rows")
-    _require(request_ids is not None or block_pool.size(0) >= batch, "block_pool has %d rows for %d sequences" % (block_pool.size(0), batch))
-    _require(block_table.size(0) == batch, "block_table has %d rows for %d sequences" % (block_table.size(0), batch))
-    _vec32(slot_mapping, slot_mapping.numel(), "slot_mapping")
-    _require(positions.dtype in (torch.int32, torch.int64) and positions.dim() == 1 and positions.is_contiguous() and
-             positions.numel() == slot_mapping.numel(), "positions must be int32 or int64, one entry per slot")
-    _require((free_blocks is None) == (free_head is None), "free_blocks and free_head go together")
-    _require(free_blocks is None or held_blocks is not None, "free_blocks needs held_blocks")
-    _require((held_blocks is None) == (held_blocks_out is None) and (held_blocks is None) == (free_head_out is None),
-             "held_blocks, held_blocks_out and free_head_out go together")
-    if free_blocks is not None:
-        _vec32(free_blocks, free_blocks.numel(), "free_blocks")
-        _vec32(free_head, 1, "free_head")
-    if free_head_out is not None:
-        _vec32(free_head_out, 2, "free_head_out")
-    csr = (paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len)
-    _require(all(t is None for t in csr) or all(t is not None for t in csr), "the paged_kv arrays go together")
-    if paged_kv_indptr is not None:
-        _vec32(paged_kv_indptr, batch + 1, "paged_kv_indptr")
-        _vec32(paged_kv_indices, paged_kv_indices.numel(), "paged_kv_indices")
-    dev = _on_gpu(cached_lens, block_pool, block_table, seq_lens, q_indptr, slot_mapping, positions, new_lens, request_ids,
-                  held_blocks, free_blocks, free_head, held_blocks_out, free_head_out, *csr)
-    a = _lib.StepArgs()
-    a.cached_lens, a.block_pool, a.block_table = cached_lens.data_ptr(), block_pool.data_ptr(), block_table.data_ptr()
-    a.seq_lens, a.q_indptr = seq_lens.data_ptr(), q_indptr.data_ptr()
-    a.slot_mapping, a.positions, a.num_rows = slot_mapping.data_ptr(), positions.data_ptr(), slot_mapping.numel()
-    a.positions_int32 = int(positions.dtype == torch.int32)
-    a.pool_rows, a.pool_width = block_pool.size(0), block_pool.size(1)
-    # (the row stride of a one-row tensor is arbitrary in torch)
-    a.pool_stride = block_pool.stride(0) if block_pool.size(0) > 1 else block_pool.size(1)
-    a.table_width = block_table.size(1)
-    a.table_stride = block_table.stride(0) if batch > 1 else block_table.size(1)
-    a.batch, a.q_per_seq, a.block_size = batch, int(q_per_seq), int(block_size)
-    if new_lens is not None:
-        a.new_lens = new_lens.data_ptr()
-    if request_ids is not None:
-        a.request_ids = request_ids.data_ptr()
-    if held_blocks is not None:
-        a.held_blocks, a.held_blocks_out, a.free_head_out = held_blocks.data_ptr(), held_blocks_out.data_ptr(), free_head_out.data_ptr()
-    if free_blocks is not None:
-        a.free_blocks, a.free_head, a.num_free = free_blocks.data_ptr(), free_head.data_ptr(), free_blocks.numel()
-    if paged_kv_indptr is not None:
-        a.kv_indptr, a.kv_indices, a.kv_last_page_len = (t.data_ptr() for t in csr)
-        a.kv_indices_capacity = paged_kv_indices.numel()
-    with _on_device(dev):
-        _lib.check(_lib.load().xllm_hip_build_step_indices(ctypes.byref(a), _stream()))
+    _shim().build_step_indices(cached_lens, block_pool, block_size, block_table, seq_lens, q_indptr, slot_mapping, positions,
+                               new_lens, q_per_seq, request_ids, held_blocks, free_blocks, free_head, held_blocks_out,
+                               free_head_out, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len)
 
 
 TREE_MAX_NODES = 512
@@ -750,32 +678,7 @@ def tree_masks(parents, tree_mask, positions=None, base=None, *, q_indptr=None, 
     or q_per_seq rows each.  tree_mask [rows, words] int64 receives a bit per ancestor (the node itself included),
     words = ceil(most nodes of a sequence / 64), at most 8; positions [rows] or [axes, rows] (int32 or int64) receives
     base[b] plus the node's depth, a child of the context having depth 0."""
-    rows = parents.numel()
-    _vec32(parents, rows, "parents")
-    _require((q_indptr is None) != (q_per_seq is None), "either q_indptr or q_per_seq")
-    if q_indptr is not None:
-        _require(q_indptr.numel() >= 1, "q_indptr must be [batch + 1]")
-        _vec32(q_indptr, q_indptr.numel(), "q_indptr")
-        batch, q_per_seq = q_indptr.numel() - 1, 0
-    else:
-        _require(q_per_seq >= 1 and rows % q_per_seq == 0, "rows not divisible by q_per_seq")
-        batch = rows // q_per_seq
-    _require(tree_mask.dtype == torch.int64 and tree_mask.dim() == 2 and tree_mask.size(0) == rows and tree_mask.size(1) >= 1 and
-             tree_mask.stride(1) == 1, "tree_mask must be int64 [rows, words], rows contiguous")
-    axes, axis_stride = 1, 0
-    if positions is not None:
-        _require(positions.dtype in (torch.int32, torch.int64) and positions.dim() in (1, 2) and positions.size(-1) == rows and
-                 (rows <= 1 or positions.stride(-1) == 1), "positions must be int32 or int64 [rows] or [axes, rows]")
-        if positions.dim() == 2:
-            axes, axis_stride = positions.size(0), positions.stride(0) if positions.size(0) > 1 else rows
-    if base is not None:
-        _vec32(base, batch, "base")
-    dev = _on_gpu(parents, tree_mask, positions, base, q_indptr)
-    with _on_device(dev):
-        _lib.check(_lib.load().xllm_hip_tree_masks(
-            parents.data_ptr(), _ptr(q_indptr), _ptr(base), batch, int(q_per_seq), rows, tree_mask.data_ptr(),
-            tree_mask.stride(0) if rows > 1 else tree_mask.size(1), tree_mask.size(1), _ptr(positions),
-            int(positions is not None and positions.dtype == torch.int32), axes, axis_stride, _stream()))
+    _shim().tree_masks(parents, tree_mask, positions, base, q_indptr, -1 if q_per_seq is None else q_per_seq)
 
 
 def mrope_kv_write(qkv, num_heads_q, num_heads_kv, head_dim, cos_sin_cache, position_ids, mrope_section, k_cache=None,
@@ -785,57 +688,13 @@ def mrope_kv_write(qkv, num_heads_q, num_heads_kv, head_dim, cos_sin_cache, posi
     mrope_section: how many rotation pairs belong to each axis (their sum is rotary_dim / 2), side by side, or with
     mrope_interleaved dealt out in turn (pair j on axis j mod axes while that axis has pairs left, else on axis 0).
     Without a cache only q and k are rewritten."""
-    _require(qkv.dim() == 2 and qkv.stride(1) == 1, "qkv must be 2-D, rows contiguous")
-    _require(qkv.size(1) >= (num_heads_q + 2 * num_heads_kv) * head_dim, "qkv rows do not hold the heads")
-    _require(position_ids.dtype in (torch.int64, torch.int32) and position_ids.dim() == 2 and
-             position_ids.size(1) == qkv.size(0) and (qkv.size(0) <= 1 or position_ids.stride(1) == 1),
-             "position_ids must be int64 or int32 [axes, tokens], rows contiguous")
-    _require(len(mrope_section) == position_ids.size(0) and 1 <= len(mrope_section) <= 4,
-             "mrope_section needs one entry for each of 1 to 4 axes")
-    _require((q_weight is None) == (k_weight is None), "q_weight and k_weight go together")
-    desc = None
-    if k_cache is not None:
-        _require(v_cache is not None and slot_mapping is not None, "k_cache needs v_cache and slot_mapping")
-        _vec32(slot_mapping, qkv.size(0), "slot_mapping")
-        desc = _cache_desc(k_cache, v_cache, k_cache_scale, v_cache_scale, kv_layout)
-    else:
-        _require(v_cache is None and slot_mapping is None, "v_cache or slot_mapping given without k_cache")
-    a = _rope_args(qkv, num_heads_q, num_heads_kv, num_heads_kv, head_dim, eps, q_weight, k_weight, cos_sin_cache,
-                   interleaved, position_ids, round_each_op)
-    m = _lib.Mrope()
-    m.num_axes, m.dealt = len(mrope_section), int(bool(mrope_interleaved))
-    m.axis_stride = position_ids.stride(0) if position_ids.size(0) > 1 else qkv.size(0)
-    for i, n in enumerate(mrope_section):
-        m.sections[i] = int(n)
-    dev = _on_gpu(qkv, cos_sin_cache, position_ids, k_cache, v_cache, slot_mapping, q_weight, k_weight, k_cache_scale,
-                  v_cache_scale)
-    with _on_device(dev):
-        _lib.check(_lib.load().xllm_hip_mrope_kv_write(ctypes.byref(a), ctypes.byref(m),
-                                                       ctypes.byref(desc) if desc is not None else None,
-                                                       _ptr(slot_mapping), _stream()))
-
-
-_tree_workspaces = {}
+    _shim().mrope_kv_write(qkv, num_heads_q, num_heads_kv, head_dim, cos_sin_cache, position_ids, mrope_section, k_cache, v_cache,
+                           slot_mapping, mrope_interleaved, q_weight, k_weight, eps, interleaved, round_each_op, k_cache_scale,
+                           v_cache_scale, _nhd(kv_layout))
 
 
 def tree_workspace_bytes(batch, q_per_seq, num_q_heads, num_kv_heads, head_dim):
     return _lib.load().xllm_hip_tree_attention_workspace_bytes(batch, q_per_seq, num_q_heads, num_kv_heads, head_dim)
-
-
-def _tree_workspace(device, nbytes):
-    """Scratch of a tree-attention call: one buffer per (device, stream) for eager calls, which grows to the largest
-    call's need, and memory of the graph's own pool for a call under capture, so that no two graphs, and no graph and
-    no eager call, share one.  (A buffer that is outgrown goes back to torch's allocator, which hands it out again in
-    the order of the stream.)"""
-    if nbytes == 0:
-        return None
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device, torch.cuda.current_stream(device).cuda_stream)
-    ws = _tree_workspaces.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = _tree_workspaces[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return ws
 
 
 def batch_tree_decode(query, k_cache, v_cache, output, block_table, seq_lens, tree_mask, *, scale, q_indptr=None,
@@ -849,31 +708,10 @@ def batch_tree_decode(query, k_cache, v_cache, output, block_table, seq_lens, tr
     indices, last_page_len) in place of block_table / seq_lens (given as None).  output_lse: float32 [tokens, Hq],
     base 2.  A row that sees nothing gets zeros and -inf."""
     _require(k_cache is not None and v_cache is not None, "k_cache and v_cache are required")
-    _require(query.dim() == 3 and output.dim() == 3, "query and output must be [tokens, heads, dim]")
-    _require(q_per_seq is not None and q_per_seq >= 1, "q_per_seq (the most query tokens of a sequence) is required")
-    _require((k_cache_quant_scale is None) == (v_cache_quant_scale is None),
-             "k_cache_quant_scale and v_cache_quant_scale go together")
-    rows = query.size(0)
-    _require(tree_mask.dtype == torch.int64 and tree_mask.dim() == 2 and tree_mask.size(0) == rows and tree_mask.size(1) >= 1 and
-             tree_mask.stride(1) == 1, "tree_mask must be int64 [tokens, words], rows contiguous")
-    _require((csr is None) == (block_table is not None) and (csr is None) == (seq_lens is not None),
-             "either block_table and seq_lens, or csr")
-    dev = _on_gpu(query, k_cache, v_cache, output, block_table, seq_lens, tree_mask, q_indptr, output_lse,
-                  k_cache_quant_scale, v_cache_quant_scale, workspace, *(csr or ()))
-    if rows == 0:
-        return
-    desc = _cache_desc(k_cache, v_cache, k_cache_quant_scale, v_cache_quant_scale, kv_layout)
-    a, _keep = _decode_args(query, output, output_lse, block_table, seq_lens, csr, q_per_seq, scale, -1, max_seq_len, desc,
-                            total_kv_len, q_indptr)
-    lib = _lib.load()
-    with _on_device(dev):
-        if workspace is None:
-            workspace = _tree_workspace(dev, lib.xllm_hip_tree_attention_workspace_bytes(
-                a.batch, a.q_per_seq, a.num_q_heads, desc.num_kv_heads, desc.head_dim))
-        wbytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
-        _lib.check(lib.xllm_hip_tree_attention(ctypes.byref(desc), ctypes.byref(a), tree_mask.data_ptr(),
-                                               tree_mask.stride(0) if rows > 1 else tree_mask.size(1), tree_mask.size(1),
-                                               _ptr(workspace), wbytes, _stream()))
+    indptr, indices, last_page_len = csr if csr is not None else (None, None, None)
+    _shim().batch_tree_decode(query, k_cache, v_cache, output, block_table, seq_lens, tree_mask, scale, q_indptr,
+                              0 if q_per_seq is None else q_per_seq, output_lse, k_cache_quant_scale, v_cache_quant_scale,
+                              _nhd(kv_layout), max_seq_len, total_kv_len, workspace, indptr, indices, last_page_len)
 
 
 def move_accepted_tokens(k_cache, v_cache, block_table, cached_lens, accepted, num_accepted, new_lens=None, *,
@@ -882,22 +720,5 @@ def move_accepted_tokens(k_cache, v_cache, block_table, cached_lens, accepted, n
     (xllm_hip_move_accepted_tokens): token cached_lens[b] + i <- token cached_lens[b] + accepted[b][i] for
     i < num_accepted[b], every row read before any is written.  accepted [batch, width] int32; new_lens [batch], if
     given, receives cached_lens + num_accepted (and must not be cached_lens itself: other layers still read it)."""
-    _require(k_cache is not None and v_cache is not None, "k_cache and v_cache are required")
-    batch = cached_lens.numel()
-    _vec32(cached_lens, batch, "cached_lens")
-    _vec32(num_accepted, batch, "num_accepted")
-    if new_lens is not None:
-        _vec32(new_lens, batch, "new_lens")
-    _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.size(0) == batch and
-             block_table.size(1) >= 1 and block_table.stride(1) == 1, "block_table must be int32 [batch, max_blocks]")
-    _require(accepted.dtype == torch.int32 and accepted.dim() == 2 and accepted.size(0) == batch and
-             (accepted.size(1) <= 1 or accepted.stride(1) == 1), "accepted must be int32 [batch, width], rows contiguous")
-    _require((k_cache_scale is None) == (v_cache_scale is None), "k_cache_scale and v_cache_scale go together")
-    dev = _on_gpu(k_cache, v_cache, block_table, cached_lens, accepted, num_accepted, new_lens, k_cache_scale, v_cache_scale)
-    desc = _cache_desc(k_cache, v_cache, k_cache_scale, v_cache_scale, kv_layout)
-    many = batch > 1
-    with _on_device(dev):
-        _lib.check(_lib.load().xllm_hip_move_accepted_tokens(
-            ctypes.byref(desc), block_table.data_ptr(), block_table.stride(0) if many else block_table.size(1),
-            block_table.size(1), cached_lens.data_ptr(), accepted.data_ptr(), accepted.stride(0) if many else accepted.size(1),
-            accepted.size(1), num_accepted.data_ptr(), batch, _ptr(new_lens), _stream()))
+    _shim().move_accepted_tokens(k_cache, v_cache, block_table, cached_lens, accepted, num_accepted, new_lens, k_cache_scale,
+                                 v_cache_scale, _nhd(kv_layout))
