@@ -160,12 +160,23 @@ static void launch_tree_merge(const TreeParams& p, hipStream_t st) {
 
 template <int QT, int KV, int D>
 static void launch_tree_mfma_d(int rows_per_item, const TreeParams& p, unsigned grid, hipStream_t st) {
+  const bool stream = p.row_groups == 1;  // nobody else reads an item's K and V
   if (rows_per_item == 32) {
-    tree_mfma_kernel<QT, KV, D, 1, 2><<<grid, 256, 0, st>>>(p);
+    tree_mfma_kernel<QT, KV, D, 1, 2, true><<<grid, 256, 0, st>>>(p);
   } else if (rows_per_item == 64) {
-    tree_mfma_kernel<QT, KV, D, 1, 1><<<grid, 256, 0, st>>>(p);
+    if (D < 256 || stream) {
+      tree_mfma_kernel<QT, KV, D, 1, 1, true><<<grid, 256, 0, st>>>(p);
+    } else {
+      if constexpr (D == 256) tree_mfma_kernel<QT, KV, D, 1, 1, false><<<grid, 256, 0, st>>>(p);
+    }
   } else {
-    if constexpr (D <= 128) tree_mfma_kernel<QT, KV, D, 2, 1><<<grid, 256, 0, st>>>(p);
+    if constexpr (D <= 128) {
+      if (stream) {
+        tree_mfma_kernel<QT, KV, D, 2, 1, true><<<grid, 256, 0, st>>>(p);
+      } else {
+        tree_mfma_kernel<QT, KV, D, 2, 1, false><<<grid, 256, 0, st>>>(p);
+      }
+    }
   }
 }
 

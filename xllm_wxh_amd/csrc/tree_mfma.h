@@ -28,6 +28,15 @@
 
 namespace xllm_hip {
 
+// 16 bytes a lane from memory into LDS.  STREAM: lines that nobody reads again are not kept (64 x 4096 tokens of bf16, 8
+// drafts: 184 -> 164 us); an item whose neighbour on the XCD reads the same K and V keeps them (32 x 8192, 512 query
+// rows to a kv head: 654 us kept, 697 streamed).
+template <bool STREAM>
+__device__ __forceinline__ void tree_to_lds(const uint8_t* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0,
+                                   STREAM ? 2 : 0);
+}
+
 constexpr bool tree_quant(int kv) { return kv == XLLM_HIP_FP8_E4M3 || kv == XLLM_HIP_INT8; }
 
 template <int QT, int KV, int D>
@@ -116,13 +125,12 @@ struct TreeLoader {
   // Byte offset of this lane's piece from the first row of a load instruction.  The rows of further instructions differ
   // in the swizzle by few bits, so few of these are distinct: K's in the row's low three bits (kVarK instructions in
   // turn), V's in the low two, or over an 8-bit cache in the group of 16.
-  static constexpr int kGroups = SH::kRW / 16;
+  static constexpr int kGroups = SH::kRW > 16 ? SH::kRW / 16 : 1;
   static constexpr int kPer = SH::kLoads / kGroups;  // load instructions per group of 16 tokens
   static constexpr int kVarK = SH::kRPI >= 8 ? 1 : 8 / SH::kRPI;
   static constexpr int kVarV = SH::kQuant ? kGroups : SH::kRPI >= 4 ? 1 : 4 / SH::kRPI;
   uint32_t off_k[kVarK], off_v[kVarV];
   int wave, lane;
-  float sc;  // the scale in flight: lanes 0..31 the K scales of the wave's tokens, 32..63 the V scales
   uint32_t sc_off;
 
   __device__ inline void init(const TreeParams& p, int w, int l) {
@@ -136,9 +144,8 @@ struct TreeLoader {
     for (int v = 0; v < kVarV; ++v) {
       off_v[v] = at + ((pos ^ tree_swz_v<SH::kRB, SH::kQuant>(w * SH::kRW + v * (SH::kQuant ? 16 : SH::kRPI) + lr)) << 4);
     }
-    sc = 0.0f;
     sc_off = 0;
-    if (SH::kQuant) sc_off = (uint32_t)((l & 15) * p.sc_stride_slot) * 4;
+    if (SH::kQuant) sc_off = (uint32_t)((l & (SH::kRW < 16 ? SH::kRW - 1 : 15)) * p.sc_stride_slot) * 4;
   }
 
   // The block that holds the wave's group g (16 tokens) of the tile at tb, by a scalar load; past the sequence's list
@@ -149,7 +156,10 @@ struct TreeLoader {
     return tree_block(p, ((const __attribute__((address_space(4))) int32_t*)it.ids)[bi]);
   }
 
-  __device__ inline void issue(const TreeParams& p, const TreeItem& it, int tb, uint8_t* stage) {
+  // The wave's loads of the tile at tb, in flight on return.  Past the sequence's end they read its last block.  `sc`:
+  // lanes 0..31 the K scales of the wave's tokens, 32..63 the V scales.
+  template <bool STREAM>
+  __device__ inline void issue(const TreeParams& p, const TreeItem& it, int tb, uint8_t* stage, float& sc) const {
     const int first = tb + wave * SH::kRW;
     uint8_t* kl = stage + wave * (SH::kRW * SH::kRB);
     uint8_t* vl = kl + SH::kArray;
@@ -169,14 +179,14 @@ struct TreeLoader {
       const uint8_t* vb = p.v_cache + elem * SH::kEB;
       const int64_t next = (int64_t)SH::kRPI * p.stride_slot * SH::kEB;  // from one instruction's rows to the next's
 #pragma unroll
-      for (int q = 0; q < kPer; ++q) XLLM_HIP_GLOBAL_TO_LDS_16(kb + q * next + off_k[q % kVarK], kl + (g * kPer + q) * 1024);
+      for (int q = 0; q < kPer; ++q) tree_to_lds<STREAM>(kb + q * next + off_k[q % kVarK], kl + (g * kPer + q) * 1024);
 #pragma unroll
       for (int q = 0; q < kPer; ++q) {
-        XLLM_HIP_GLOBAL_TO_LDS_16(vb + q * next + off_v[SH::kQuant ? g : q % kVarV], vl + (g * kPer + q) * 1024);
+        tree_to_lds<STREAM>(vb + q * next + off_v[SH::kQuant ? g : q % kVarV], vl + (g * kPer + q) * 1024);
       }
     }
     if constexpr (SH::kQuant) {
-      // lane = (array, token among the wave's, 16 of them twice where there are only 16)
+      // lane = (array, token among the wave's, several times where there are fewer than 32)
       const int64_t sb = kGroups > 1 && (lane & 16) != 0 ? sbase[kGroups - 1] : sbase[0];
       const float* arr = (lane & 32) != 0 ? p.v_scale : p.k_scale;
       sc = *(const float*)((const uint8_t*)(arr + sb) + sc_off);
@@ -188,7 +198,7 @@ struct TreeLoader {
   //   lv   = log2 v_scale                      weight 2^(x - max x): the V scale rides in the exponent, so the 16-bit
   //   rvs  = 1 / v_scale                       weights use their whole range; a weight's share of the sum is w * rvs
   // A V scale of 0 counts as 2^-100: its tokens keep their share of the sum and add nothing.
-  __device__ inline void factors(const TreeParams& p, uint8_t* stage) const {
+  __device__ inline void factors(const TreeParams& p, uint8_t* stage, float sc) const {
     if constexpr (SH::kQuant) {
       float* f = (float*)(stage + SH::kFactors);
       const int i = lane & 31;
@@ -231,32 +241,32 @@ __device__ inline int tree_row(const TreeParams& p, const TreeItem& it, int firs
   return row < it.n * p.group ? row : -1;
 }
 
-// The mask of the lane's row.
+// The mask of the lane's row.  KEEP: its first word is held in registers (fetched while the last tiles are in flight);
+// otherwise, and for the further words of trees of more than 64 nodes, words are fetched by the pieces that need them.
+template <bool KEEP>
 struct TreeRowMask {
-  const uint64_t* mask;
   uint64_t word0;
-  int words;  // 0 where the lane has no row
 
-  __device__ inline void init(const TreeParams& p, const TreeItem& it, int first_row, int lane) {
+  __device__ static inline uint64_t word(const TreeParams& p, const TreeItem& it, int first_row, int lane, int w) {
     const int row = tree_row(p, it, first_row, lane);
-    mask = p.mask + (it.q0 + (row < 0 ? 0 : row) / p.group) * p.mask_stride;
-    words = row < 0 ? 0 : p.mask_words;
-    word0 = row < 0 ? 0 : mask[0];
+    if (row < 0 || w >= p.mask_words) return 0;
+    return p.mask[(it.q0 + row / p.group) * p.mask_stride + w];
   }
-
+  __device__ inline void init(const TreeParams& p, const TreeItem& it, int first_row, int lane) {
+    if (KEEP) word0 = word(p, it, first_row, lane, 0);
+  }
   // Bits of the 32 tokens from t0 on that the row sees.
-  __device__ inline uint32_t bits(const TreeItem& it, int t0) const {
+  __device__ inline uint32_t bits(const TreeParams& p, const TreeItem& it, int first_row, int lane, int t0) const {
     uint32_t b;
     const int u = t0 - it.prefix;
     if (u <= -32) {
       b = ~0u;
     } else if (u < 0) {  // the context's last tokens, then the first drafted ones
-      b = (uint32_t)(word0 << -u) | ((1u << -u) - 1u);
+      b = (uint32_t)((KEEP ? word0 : word(p, it, first_row, lane, 0)) << -u) | ((1u << -u) - 1u);
     } else {
       const int w = u >> 6, s = u & 63;
-      const uint64_t lo = w == 0 ? word0 : (w < words ? mask[w] : 0);
-      uint64_t v = lo >> s;
-      if (s > 32 && w + 1 < words) v |= mask[w + 1] << (64 - s);
+      uint64_t v = (KEEP && w == 0 ? word0 : word(p, it, first_row, lane, w)) >> s;
+      if (s > 32) v |= word(p, it, first_row, lane, w + 1) << (64 - s);
       b = (uint32_t)v;
     }
     const int left = it.len - t0;
@@ -381,8 +391,10 @@ struct TreeRows {
   }
 };
 
-// RTW: row tiles per wave; TS: waves that share a row tile's tokens (2 with RTW = 1, else 1).
-template <int QT, int KV, int D, int RTW, int TS>
+// RTW: row tiles per wave; TS: waves that share a row tile's tokens (2 with RTW = 1, else 1); STREAM: see tree_to_lds
+// (one row group; a template argument, because a branch in the loop costs the compiler its schedule: 24 fp8 sequences, 61
+// drafts, 379 against 353 us).
+template <int QT, int KV, int D, int RTW, int TS, bool STREAM>
 __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1 : 2)) tree_mfma_kernel(TreeParams p) {
   typedef TreeShape<QT, KV, D> SH;
   static_assert(TS == 1 || (TS == 2 && RTW == 1), "two waves share one row tile at most");
@@ -410,7 +422,8 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
   ld.init(p, wave, lane);
   const int t0 = it.t_begin;
   const int iters = it.t_end > t0 ? (it.t_end - t0 + SH::kTT - 1) / SH::kTT : 0;
-  if (iters > 0) ld.issue(p, it, t0, stage0);
+  float sc = 0.0f;  // the scales in flight (8-bit caches)
+  if (iters > 0) ld.template issue<STREAM>(p, it, t0, stage0, sc);
 
   TreeRows<SH, KV> rows[RTW];
 #pragma unroll
@@ -492,7 +505,7 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
   };
 
   // 32 tokens: those every row sees, or (MASKED) under the rows' bits.
-  TreeRowMask masks[RTW];
+  TreeRowMask<RTW == 1 || SH::kQuant> masks[RTW];
   auto attend = [&](const uint8_t* stage, int tb, int piece, auto masked) {
     constexpr bool MASKED = decltype(masked)::value;
     const uint8_t* tile = stage + piece * SH::kRB;
@@ -500,7 +513,7 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
     scores(tile, std::integral_constant<int, RTW>{}, 0, s);
     uint32_t vis[RTW];
 #pragma unroll
-    for (int a = 0; a < RTW; ++a) vis[a] = MASKED ? masks[a].bits(it, tb + piece) : 0u;
+    for (int a = 0; a < RTW; ++a) vis[a] = MASKED ? masks[a].bits(p, it, first_row + 16 * a, lane, tb + piece) : 0u;
     float x[RTW][8];
     {
       f32x4 kscl[2], lv[2];
@@ -545,7 +558,7 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
     for (int a = 0; a < RTW; ++a) {
       f32x4 s[1][2];
       scores(tile, std::integral_constant<int, 1>{}, a, s);
-      const uint32_t vis = masks[a].bits(it, tb + piece);
+      const uint32_t vis = masks[a].bits(p, it, first_row + 16 * a, lane, tb + piece);
       float w[8], alpha;
       {
         f32x4 kscl[2], lv[2];
@@ -583,12 +596,14 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
   // Tile i from `here`: its loads have landed (every wave waits for its own), the waves meet — nobody reads `next` any
   // more — tile i + 1 goes in flight into `next`, tile i is attended.  The two stages are LDS arrays of their own and
   // the loop over tiles that every row sees is written out for both, so that the compiler can tell the loads in
-  // flight from the tile being read and does not wait for them.
+  // flight from the tile being read and does not wait for them.  (Four stages of half the tokens, three of them in
+  // flight, were slower: 24 fp8 sequences, 61 drafts, 413 against 353 us; 64 x 4096 bf16 tokens 193 against 184: what
+  // a step costs beside its tokens outweighs the deeper queue.)
   auto step = [&](int i, uint8_t* here, uint8_t* next) {
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    ld.factors(p, here);
+    ld.factors(p, here, sc);
     __syncthreads();
-    if (i + 1 < iters) ld.issue(p, it, t0 + (i + 1) * SH::kTT, next);
+    if (i + 1 < iters) ld.template issue<STREAM>(p, it, t0 + (i + 1) * SH::kTT, next, sc);
     if (!has_rows) return;
 #pragma unroll 1
     for (int piece = 32 * tg; piece < SH::kTT; piece += 32 * TS) attend(here, 0, piece, std::false_type{});
@@ -600,8 +615,7 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
     step(i, stage0, stage1);
     step(i + 1, stage1, stage0);
   }
-  // The rest: an odd tile of the context, the last of the context with the drafted tokens behind it, and so on.  (The
-  // masks are fetched only here: two row tiles have no registers for them in the loop above.)
+  // The rest: an odd tile of the context, the last of the context with the drafted tokens behind it, and so on.
   if (i < iters) {
 #pragma unroll
     for (int a = 0; a < RTW; ++a) masks[a].init(p, it, first_row + 16 * a, lane);
@@ -610,14 +624,14 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
     uint8_t* here = (i & 1) != 0 ? stage1 : stage0;
     const int tb = t0 + i * SH::kTT;
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    ld.factors(p, here);
+    ld.factors(p, here, sc);
     const bool masked = tb + SH::kTT > it.prefix;
     if (KV != XLLM_HIP_INT8 && masked) {
       const bool bad = ld.look_through(tb, it.prefix, it.len, here);
       if (lane == 0) found[i & 1][wave] = bad;
     }
     __syncthreads();  // (factors, zeros and findings are in LDS too)
-    if (i + 1 < iters) ld.issue(p, it, tb + SH::kTT, (i & 1) != 0 ? stage0 : stage1);
+    if (i + 1 < iters) ld.template issue<STREAM>(p, it, tb + SH::kTT, (i & 1) != 0 ? stage0 : stage1, sc);
     if (!has_rows) continue;
     bool exact = false;
     if (KV != XLLM_HIP_INT8 && masked) {
@@ -636,22 +650,24 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
     }
   }
 
-  // End of the item.
+  // End of the item.  (The lane's number is formed anew: held through the loops it costs a register.)
+  const int end_lane = lane_id(), end_kg = end_lane >> 4;
   const float neg_inf = -INFINITY;
   if constexpr (TS == 2) {
     // the second wave of a row tile hands over its sums; nothing is in flight any more
     __syncthreads();
     uint8_t* xch = (wave & 1) != 0 ? stage1 : stage0;
+    float* ml = (float*)(xch + SH::kDT * 1024);
     Rows& r = rows[0];
     if (tg == 1) {
-      *(float*)(xch + lane * 4) = r.m_run;
-      *(float*)(xch + 256 + lane * 4) = r.l_run;
+      ml[end_lane] = r.m_run;
+      ml[64 + end_lane] = r.l_run;
 #pragma unroll
-      for (int dt = 0; dt < SH::kDT; ++dt) *(f32x4*)(xch + 512 + dt * 1024 + lane * 16) = r.acc[dt];
+      for (int dt = 0; dt < SH::kDT; ++dt) *(f32x4*)(xch + dt * 1024 + end_lane * 16) = r.acc[dt];
     }
     __syncthreads();
     if (tg == 1) return;
-    const float m2 = *(const float*)(xch + lane * 4), l2 = *(const float*)(xch + 256 + lane * 4);
+    const float m2 = ml[end_lane], l2 = ml[64 + end_lane];
     const float m = fmaxf(r.m_run, m2);
     const float m_safe = m == neg_inf ? 0.0f : m;
     const float a1 = __builtin_amdgcn_exp2f(r.m_run - m_safe), a2 = __builtin_amdgcn_exp2f(m2 - m_safe);
@@ -659,7 +675,7 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
     r.l_run = r.l_run * a1 + l2 * a2;
 #pragma unroll
     for (int dt = 0; dt < SH::kDT; ++dt) {
-      const f32x4 o = *(const f32x4*)(xch + 512 + dt * 1024 + lane * 16);
+      const f32x4 o = *(const f32x4*)(xch + dt * 1024 + end_lane * 16);
       r.acc[dt] = r.acc[dt] * a1 + o * a2;
     }
   }
@@ -668,7 +684,7 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
   for (int a = 0; a < RTW; ++a) {
     Rows& r = rows[a];
     const float l = kg_sum(r.l_run);
-    const int row = tree_row(p, it, first_row + 16 * a, lane);
+    const int row = tree_row(p, it, first_row + 16 * a, end_lane);
     if (row < 0) continue;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a NaN stays one)
     const float lse2 = l == 0.0f ? neg_inf : r.m_run + __builtin_amdgcn_logf(l);
@@ -676,8 +692,8 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
     const int head = it.hk * p.group + (row - j * p.group);
     const int64_t token = it.q0 + j;
     if (it.chunks == 1) {
-      if (kg == 0 && p.lse != nullptr) p.lse[token * p.num_q_heads + head] = lse2;
-      uint16_t* out = (uint16_t*)p.out + token * p.out_token_stride + (int64_t)head * D + 4 * kg;
+      if (end_kg == 0 && p.lse != nullptr) p.lse[token * p.num_q_heads + head] = lse2;
+      uint16_t* out = (uint16_t*)p.out + token * p.out_token_stride + (int64_t)head * D + 4 * end_kg;
 #pragma unroll
       for (int dt = 0; dt < SH::kDT; ++dt) {
         const f32x4 o = r.acc[dt] * inv;
@@ -686,8 +702,8 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
       }
     } else {
       const int64_t prow = ((int64_t)it.b * p.slots + it.chunk) * ((int64_t)p.n * p.num_q_heads) + (int64_t)j * p.num_q_heads + head;
-      if (kg == 0) p.partial_lse[prow] = lse2;
-      float* out = p.partial_out + prow * D + 4 * kg;
+      if (end_kg == 0) p.partial_lse[prow] = lse2;
+      float* out = p.partial_out + prow * D + 4 * end_kg;
 #pragma unroll
       for (int dt = 0; dt < SH::kDT; ++dt) *(f32x4*)(out + dt * 16) = r.acc[dt] * inv;
     }
