@@ -65,12 +65,11 @@ static void launch_tree_generic(int kv_dt, const TreeParams& p, unsigned grid, h
 // How the matrix kernels would run a call; rows_per_item 0: they do not serve it.
 struct TreeForm {
   int rows_per_item;
-  int tile;
   int slots;  // workgroups that run at a time on 256 CUs
 };
 
 static TreeForm tree_form(const xllm_hip_kv_cache* c, const xllm_hip_decode_args* a) {
-  TreeForm none{0, 64, 0};
+  TreeForm none{0, 0};
   const int eb = elem_bytes(c->dtype);
   const bool quant = c->dtype == XLLM_HIP_FP8_E4M3 || c->dtype == XLLM_HIP_INT8;
   if (a->q_dtype != XLLM_HIP_BF16 && a->q_dtype != XLLM_HIP_FP16) return none;
@@ -89,7 +88,6 @@ static TreeForm tree_form(const xllm_hip_kv_cache* c, const xllm_hip_decode_args
   const int rb = c->head_dim * eb;
   TreeForm f;
   f.rows_per_item = rows <= 32 ? 32 : (rows <= 64 || c->head_dim == 256) ? 64 : 128;
-  f.tile = rb >= 256 ? 64 : 128;
   f.slots = rb == 512 ? 256 : 512;
   return f;
 }
@@ -146,15 +144,24 @@ static void choose_chunks(const xllm_hip_decode_args* a, const TreeForm& form, i
   p.slots = best_cut;
 }
 
+template <int Q_DT, int COLS>
+static void launch_tree_merge_cols(const TreeParams& p, hipStream_t st) {
+  const int rows = p.n * p.num_q_heads;  // (p.n <= kTreeMaxNodes)
+  if ((int64_t)p.batch * rows <= 8192) {  // two waves to a CU's SIMD
+    tree_merge_kernel<Q_DT, COLS, 1><<<dim3((unsigned)((rows + 3) / 4), (unsigned)p.batch), 256, 0, st>>>(p);
+  } else {
+    tree_merge_kernel<Q_DT, COLS, 4><<<dim3((unsigned)((rows + 15) / 16), (unsigned)p.batch), 256, 0, st>>>(p);
+  }
+}
+
 template <int Q_DT>
 static void launch_tree_merge(const TreeParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)((p.n * p.num_q_heads + 15) / 16), (unsigned)p.batch);
   if (p.head_dim <= 64) {
-    tree_merge_kernel<Q_DT, 16><<<grid, 256, 0, st>>>(p);
+    launch_tree_merge_cols<Q_DT, 16>(p, st);
   } else if (p.head_dim <= 128) {
-    tree_merge_kernel<Q_DT, 32><<<grid, 256, 0, st>>>(p);
+    launch_tree_merge_cols<Q_DT, 32>(p, st);
   } else {
-    tree_merge_kernel<Q_DT, 64><<<grid, 256, 0, st>>>(p);
+    launch_tree_merge_cols<Q_DT, 64>(p, st);
   }
 }
 
@@ -316,7 +323,7 @@ extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
     p.partial_out = (float*)((uint8_t*)workspace + tree_lse_bytes(a->batch, p.n, p.num_q_heads, slots));
   }
   const TreeForm form = tree_form(c, a);
-  p.tile = form.tile;
+  p.tile = form.rows_per_item > 0 ? 32 : 64;  // (what the kernels take at a time)
   const int64_t rows = (int64_t)p.n * p.group;
   p.row_groups = (int32_t)(form.rows_per_item > 0 ? (rows + form.rows_per_item - 1) / form.rows_per_item : rows);
   choose_chunks(a, form, elem_bytes(c->dtype), p);

@@ -93,14 +93,15 @@ __global__ void __launch_bounds__(64) tree_generic_kernel(TreeParams p) {
 
 // Rows of cut sequences: out = sum_c 2^(lse_c - lse) partial_c, lse = log2 sum_c 2^lse_c; a chunk that saw nothing has
 // lse -inf, weight 0 and a partial of zeros.  Bound by the partials' bytes and by the latency of their loads, so four
-// floats to a lane, D / 4 lanes to a chunk's row (a wave has 64 / (D / 4) chunks' rows at a time), and four query rows
-// to a wave, whose loads all go out before the first is used.
-template <int Q_DT, int COLS>
+// floats to a lane, D / 4 lanes to a chunk's row (a wave has 64 / (D / 4) chunks' rows at a time), and ROWS query rows
+// to a wave, all of whose loads go out before the first is used: four where there are rows enough, else one, with more
+// of its chunks at a time.
+template <int Q_DT, int COLS, int ROWS>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
   static_assert(COLS == 16 || COLS == 32 || COLS == 64, "lanes that share a chunk's row, four columns each");
   constexpr int kAtOnce = 64 / COLS;
-  constexpr int kUnroll = COLS == 64 ? 4 : 2;  // loads per query row in flight
-  constexpr int kRows = 4;
+  constexpr int kRows = ROWS;
+  constexpr int kUnroll = (ROWS == 1 ? 8 : 2) * (COLS == 64 ? 2 : 1);  // loads per query row in flight
   const int lane = threadIdx.x & 63;
   // (grid: rows of a sequence, sequences; the workgroups of a sequence that was not cut end here)
   const int b = blockIdx.y;

@@ -455,11 +455,13 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
   // The operands of 32 tokens: K rows 16h + mi, elements of chunk c (16-bit), or chunks 2c and 2c + 1 (8-bit) ...
   auto k_operand = [&](const uint8_t* tile, uint32_t ko, int c, int h) { return *(const u32x4*)(tile + (ko ^ (uint32_t)(c << 6)) + h * 16 * SH::kRB); };
   // ... and V^T, head-dim tile dt.
+  typedef __attribute__((ext_vector_type(2))) int i32x2;
+  auto v_bytes = [&](const uint8_t* tile, uint32_t vo, int dt) {
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(tile + (vo ^ (uint32_t)(dt << 4))));
+  };
   auto v_operand = [&](const uint8_t* tile, uint32_t vo, int dt) {
     if constexpr (SH::kQuant) {
-      typedef __attribute__((ext_vector_type(2))) int i32x2;
-      const i32x2 raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-          (__attribute__((address_space(3))) i32x2*)(tile + (vo ^ (uint32_t)(dt << 4))));
+      const i32x2 raw = v_bytes(tile, vo, dt);
       return __builtin_bit_cast(OpV, tree_widen<KV, SH::kVF16>((uint32_t)raw[0], (uint32_t)raw[1]));
     } else {
       const uint32_t at = vo ^ (uint32_t)(dt << 5);
@@ -505,7 +507,7 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
   };
 
   // 32 tokens: those every row sees, or (MASKED) under the rows' bits.
-  TreeRowMask<RTW == 1 || SH::kQuant> masks[RTW];
+  TreeRowMask<RTW == 1> masks[RTW];
   auto attend = [&](const uint8_t* stage, int tb, int piece, auto masked) {
     constexpr bool MASKED = decltype(masked)::value;
     const uint8_t* tile = stage + piece * SH::kRB;
@@ -522,10 +524,19 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
 #pragma unroll
       for (int a = 0; a < RTW; ++a) rows[a].template scaled<MASKED>(s[a], kscl, lv, p.scale_log2, vis[a], kg, x[a]);
     }
-    // (the factors live as briefly as they can: two row tiles leave no register to spare)
-    if (SH::kQuant && RTW > 1) __builtin_amdgcn_sched_barrier(0);
+    // Two row tiles over an 8-bit cache leave no register to spare: the factors live as briefly as they can, and the
+    // registers they leave take V's bytes, which are on their way while the weights are formed.
+    constexpr bool kAhead = SH::kQuant && RTW > 1;
+    if (kAhead) __builtin_amdgcn_sched_barrier(0);
     f32x4 rvs[2];
     factor(stage, piece, 2, rvs);
+    const uint32_t vo = fresh(v_off);
+    i32x2 vraw[kAhead ? SH::kDT : 1];
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int dt = 0; dt < SH::kDT; ++dt) vraw[dt] = v_bytes(tile, vo, dt);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     OpV pf[RTW];
     float alpha[RTW];
     bool moved = false;
@@ -541,10 +552,14 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
         for (int dt = 0; dt < SH::kDT; ++dt) rows[a].acc[dt] *= alpha[a];
       }
     }
-    const uint32_t vo = fresh(v_off);
 #pragma unroll
     for (int dt = 0; dt < SH::kDT; ++dt) {
-      const OpV vf = v_operand(tile, vo, dt);
+      OpV vf;
+      if constexpr (kAhead) {
+        vf = __builtin_bit_cast(OpV, tree_widen<KV, SH::kVF16>((uint32_t)vraw[dt][0], (uint32_t)vraw[dt][1]));
+      } else {
+        vf = v_operand(tile, vo, dt);
+      }
 #pragma unroll
       for (int a = 0; a < RTW; ++a) rows[a].acc[dt] = MmaOps<SH::kVF16>::run(vf, pf[a], rows[a].acc[dt]);
     }
@@ -608,8 +623,8 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
 #pragma unroll 1
     for (int piece = 32 * tg; piece < SH::kTT; piece += 32 * TS) attend(here, 0, piece, std::false_type{});
   };
-  // Tiles whose tokens all lie in the context, and within the length.
-  const int whole = it.prefix > t0 ? min((it.prefix - t0) / SH::kTT, iters) : 0;
+  // Tiles of the chunk whose tokens all lie in the context.
+  const int whole = max(min(it.prefix, it.t_end) - t0, 0) / SH::kTT;
   int i = 0;
   for (; i + 2 <= whole; i += 2) {
     step(i, stage0, stage1);
