@@ -159,6 +159,8 @@ def test_move_refusals(lib):
     refused(lib, _lib.INVALID_ARGUMENT, "accepted shape", call(acc_stride=4))
     refused(lib, _lib.INVALID_ARGUMENT, "overlaps cached_lens", call(new=0x2004))
     refused(lib, _lib.INVALID_ARGUMENT, "overlaps num_accepted", call(new=0x4000))
+    refused(lib, _lib.INVALID_ARGUMENT, "overlaps accepted", call(new=0x3000 + 4 * 9))
+    refused(lib, _lib.INVALID_ARGUMENT, "overlaps block_table", call(new=0x1000 + 4 * 7))
     refused(lib, _lib.INVALID_ARGUMENT, "needs k_scale", call(cache=kv_desc(_lib.INT8)))
     assert call(batch=0) == _lib.OK
 

