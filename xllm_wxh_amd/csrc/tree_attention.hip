@@ -169,7 +169,8 @@ template <int QT, int KV, int D>
 static void launch_tree_mfma_d(int rows_per_item, const TreeParams& p, unsigned grid, hipStream_t st) {
   const bool stream = p.row_groups == 1;  // nobody else reads an item's K and V
   if (rows_per_item == 32) {
-    tree_mfma_kernel<QT, KV, D, 1, 2, true><<<grid, 256, 0, st>>>(p);
+    constexpr bool kBoth = tree_quant(KV) && D <= 128;  // (two row tiles of head_dim 256 do not fit the registers)
+    tree_mfma_kernel<QT, KV, D, kBoth ? 2 : 1, kBoth ? 4 : 2, true><<<grid, 256, 0, st>>>(p);
   } else if (rows_per_item == 64) {
     if (D < 256 || stream) {
       tree_mfma_kernel<QT, KV, D, 1, 1, true><<<grid, 256, 0, st>>>(p);

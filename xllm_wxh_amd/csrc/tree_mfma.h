@@ -13,7 +13,8 @@
 // With V in fp16 the weights of an 8-bit cache are rounded to 11 bits, those over a bf16 cache to 8.
 //
 // How the waves share an item: 64 rows or 128 rows to a workgroup are 16 or 32 to each wave, which then reads all of
-// the tile; up to 32 rows are two tiles of 16, and two waves share a row tile, taking alternate 32-token pieces.  The
+// the tile.  Up to 32 rows are two tiles of 16: over a 16-bit cache two waves share a row tile, taking alternate 32-token
+// pieces; over an 8-bit cache each wave has both row tiles and every fourth piece, so that a piece is widened once.  The
 // second half of such an item's arithmetic is often unused (16 rows or fewer): a step this narrow is bound by memory.
 //
 // Only the last tokens of a sequence are drafted ones, so only the last pieces are masked.  There a row takes from its
@@ -391,18 +392,58 @@ struct TreeRows {
   }
 };
 
-// RTW: row tiles per wave; TS: waves that share a row tile's tokens (2 with RTW = 1, else 1); STREAM: see tree_to_lds
+// Where the lane's row goes: the output, or (cut sequences) a normalised partial and its base-2 log-sum-exp.
+struct TreeOut {
+  float* partial;
+  uint16_t* out;
+  float inv;
+
+  // `l`, `m`: the row's sum and reference point.  False: the lane has no row.
+  __device__ inline bool init(const TreeParams& p, const TreeItem& it, int first_row, int lane, float l, float m, bool writes_lse) {
+    const int row = tree_row(p, it, first_row, lane);
+    if (row < 0) return false;
+    inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a NaN stays one)
+    const float lse2 = l == 0.0f ? -INFINITY : m + __builtin_amdgcn_logf(l);
+    const int j = row / p.group;
+    const int head = it.hk * p.group + (row - j * p.group);
+    partial = nullptr;
+    if (it.chunks == 1) {
+      const int64_t token = it.q0 + j;
+      if (writes_lse && p.lse != nullptr) p.lse[token * p.num_q_heads + head] = lse2;
+      out = (uint16_t*)p.out + token * p.out_token_stride + (int64_t)head * p.head_dim;
+    } else {
+      const int64_t prow = ((int64_t)it.b * p.slots + it.chunk) * ((int64_t)p.n * p.num_q_heads) + (int64_t)j * p.num_q_heads + head;
+      if (writes_lse) p.partial_lse[prow] = lse2;
+      partial = p.partial_out + prow * p.head_dim;
+    }
+    return true;
+  }
+  template <bool F16>
+  __device__ inline void store(int d, f32x4 o) const {
+    o *= inv;
+    if (partial != nullptr) {
+      *(f32x4*)(partial + d) = o;
+    } else {
+      typedef MmaOps<F16> M;
+      *(u32x2*)(out + d) = u32x2{M::pack(o[0], o[1]), M::pack(o[2], o[3])};
+    }
+  }
+};
+
+// RTW: row tiles per wave; TS: waves that share the tokens of a set of row tiles, a 32-token piece each in turn; STREAM: see tree_to_lds
 // (one row group; a template argument, because a branch in the loop costs the compiler its schedule: 24 fp8 sequences, 61
 // drafts, 379 against 353 us).
 template <int QT, int KV, int D, int RTW, int TS, bool STREAM>
 __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1 : 2)) tree_mfma_kernel(TreeParams p) {
   typedef TreeShape<QT, KV, D> SH;
-  static_assert(TS == 1 || (TS == 2 && RTW == 1), "two waves share one row tile at most");
+  static_assert(TS == 1 || (TS == 2 && RTW == 1) || TS == 4, "how the end of the item joins the waves' sums");
   constexpr int kRowsPerItem = 16 * RTW * 4 / TS;
+  constexpr int kSums = RTW * SH::kDT * 1024;  // bytes of a wave's accumulators
   __shared__ __attribute__((aligned(16))) uint8_t stage0[SH::kStage];
   __shared__ __attribute__((aligned(16))) uint8_t stage1[SH::kStage];
   __shared__ int found[2][4];  // per stage and wave: a masked tile's V rows hold something that is not finite
-  static_assert(SH::kDT * 1024 + 512 <= SH::kStage, "the exchange of two waves must fit a stage");
+  __shared__ float lds_ml[TS == 4 ? 4 * RTW * 32 : 1];
+  static_assert(TS == 1 || (TS == 2 ? SH::kDT * 1024 + 512 : 2 * kSums) <= SH::kStage, "the exchange of the waves must fit the stages");
 
   TreeItem it;
   int id = blockIdx.x;
@@ -415,8 +456,8 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int mi = lane & 15, kg = lane >> 4;
-  const int tg = TS == 2 ? wave >> 1 : 0;                        // which of the two waves of the row tile
-  const int first_row = it.rg * kRowsPerItem + (TS == 2 ? wave & 1 : wave * RTW) * 16;
+  const int tg = TS == 4 ? wave : TS == 2 ? wave >> 1 : 0;  // which of the waves that share the tokens
+  const int first_row = it.rg * kRowsPerItem + (TS == 4 ? 0 : TS == 2 ? wave & 1 : wave * RTW) * 16;
 
   TreeLoader<SH, KV> ld;
   ld.init(p, wave, lane);
@@ -694,34 +735,57 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
       r.acc[dt] = r.acc[dt] * a1 + o * a2;
     }
   }
+  if constexpr (TS == 4) {
+    // All four hand over their sums; each finishes a quarter of the head's columns.
+    __syncthreads();
+    const int end_mi = end_lane & 15;
+    uint8_t* mine = (wave < 2 ? stage0 : stage1) + (wave & 1) * kSums;
+#pragma unroll
+    for (int a = 0; a < RTW; ++a) {
+      const float l = kg_sum(rows[a].l_run);
+      if (end_kg == 0) {
+        lds_ml[(wave * RTW + a) * 32 + end_mi] = rows[a].m_run;
+        lds_ml[(wave * RTW + a) * 32 + 16 + end_mi] = l;
+      }
+#pragma unroll
+      for (int dt = 0; dt < SH::kDT; ++dt) *(f32x4*)(mine + (a * SH::kDT + dt) * 1024 + end_lane * 16) = rows[a].acc[dt];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int a = 0; a < RTW; ++a) {
+      float m = neg_inf, l = 0.0f, w[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) m = fmaxf(m, lds_ml[(x * RTW + a) * 32 + end_mi]);
+      const float m_safe = m == neg_inf ? 0.0f : m;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        w[x] = __builtin_amdgcn_exp2f(lds_ml[(x * RTW + a) * 32 + end_mi] - m_safe);
+        l += w[x] * lds_ml[(x * RTW + a) * 32 + 16 + end_mi];
+      }
+      TreeOut out;
+      if (!out.init(p, it, first_row + 16 * a, end_lane, l, m, wave == 0 && end_kg == 0)) continue;
+#pragma unroll
+      for (int q = 0; q < SH::kDT / 4; ++q) {
+        const int dt = wave * (SH::kDT / 4) + q;
+        f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          o += w[x] * *(const f32x4*)((x < 2 ? stage0 : stage1) + (x & 1) * kSums + (a * SH::kDT + dt) * 1024 + end_lane * 16);
+        }
+        out.template store<SH::kQF16>(dt * 16 + 4 * end_kg, o);
+      }
+    }
+    return;
+  }
   if (!has_rows) return;
 #pragma unroll
   for (int a = 0; a < RTW; ++a) {
     Rows& r = rows[a];
     const float l = kg_sum(r.l_run);
-    const int row = tree_row(p, it, first_row + 16 * a, end_lane);
-    if (row < 0) continue;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a NaN stays one)
-    const float lse2 = l == 0.0f ? neg_inf : r.m_run + __builtin_amdgcn_logf(l);
-    const int j = row / p.group;
-    const int head = it.hk * p.group + (row - j * p.group);
-    const int64_t token = it.q0 + j;
-    if (it.chunks == 1) {
-      if (end_kg == 0 && p.lse != nullptr) p.lse[token * p.num_q_heads + head] = lse2;
-      uint16_t* out = (uint16_t*)p.out + token * p.out_token_stride + (int64_t)head * D + 4 * end_kg;
+    TreeOut out;
+    if (!out.init(p, it, first_row + 16 * a, end_lane, l, r.m_run, end_kg == 0)) continue;
 #pragma unroll
-      for (int dt = 0; dt < SH::kDT; ++dt) {
-        const f32x4 o = r.acc[dt] * inv;
-        typedef MmaOps<SH::kQF16> M;
-        *(u32x2*)(out + dt * 16) = u32x2{M::pack(o[0], o[1]), M::pack(o[2], o[3])};
-      }
-    } else {
-      const int64_t prow = ((int64_t)it.b * p.slots + it.chunk) * ((int64_t)p.n * p.num_q_heads) + (int64_t)j * p.num_q_heads + head;
-      if (end_kg == 0) p.partial_lse[prow] = lse2;
-      float* out = p.partial_out + prow * D + 4 * end_kg;
-#pragma unroll
-      for (int dt = 0; dt < SH::kDT; ++dt) *(f32x4*)(out + dt * 16) = r.acc[dt] * inv;
-    }
+    for (int dt = 0; dt < SH::kDT; ++dt) out.template store<SH::kQF16>(dt * 16 + 4 * end_kg, r.acc[dt]);
   }
 }
 
