@@ -148,6 +148,21 @@ def test_nhd_and_large_trees(gpu, kv, layout):
     c.check(*c.run())
 
 
+@pytest.mark.parametrize("q", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,spread", [(6, 1.0), (24, 1.0), (40, 2.0 ** -20)])
+def test_int8_scores_of_queries_with_a_common_sign(gpu, q, n, spread):
+    """The kernels may hold int8 keys with an offset of 128, which the sum of the query's elements takes back: the most that
+    has to cancel is there when all of them have one sign.  (The bound is the file's: (D + 8) 2^-24 sum |q k| with |k| of
+    about 40 steps leaves 128 sum |q| some 40 roundings.)  `spread`: rows far smaller than others of the same kv head."""
+    c = TreeCase([n, n - 1], [700, 64], 8, 2, 128, 16, q=q, kv="int8", seed=n)
+    mags = torch.abs(c.q.float())
+    mags[1::2] *= spread
+    c.q = mags.to(c.q.dtype)
+    c.q_ref = c.q.float().cpu().numpy()
+    out, lse = c.run()
+    c.check(out, lse)
+
+
 @pytest.mark.parametrize("D,bs,kv", [(80, 16, "bf16"), (128, 24, "bf16"), (64, 16, "int8"), (128, 8, "fp8"), (96, 5, "fp32")])
 def test_shapes_off_the_matrix_path(gpu, D, bs, kv):
     print("case tree generic", D, bs, kv, flush=True)

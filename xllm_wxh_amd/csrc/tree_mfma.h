@@ -9,7 +9,10 @@
 // after the one in use always in flight; an 8-bit cache stays bytes there — half the LDS traffic — and becomes 16-bit
 // operands in the registers that feed the matrix instructions:
 //   fp8   K to the queries' type, V to fp16, both exact
-//   int8  x ^ 0x80 = x + 128 placed behind 0x64 is the fp16 number 1024 + 128 + x; minus 1152 it is x, exactly
+//   int8  x ^ 0x80 = x + 128.  V: behind 0x64 it is the fp16 number 1024 + 128 + x; minus 1152 it is x, exactly.  K: behind
+//         0 it is the subnormal (x + 128) 2^-24, and the row takes back 128 times the sum of its query's elements with
+//         the factor that its scores get anyway.  (Twice 128 is the most that this adds to a product, so the fp32 sums
+//         lose about a bit.  V has no such end: there the 128 would pile up over the tokens.)
 // With V in fp16 the weights of an 8-bit cache are rounded to 11 bits, those over a bf16 cache to 8.
 //
 // How the waves share an item: 64 rows or 128 rows to a workgroup are 16 or 32 to each wave, which then reads all of
@@ -100,6 +103,18 @@ __device__ inline u32x4 tree_widen(uint32_t a, uint32_t b) {
     }
   }
   return o;
+}
+
+// The same for the K operand of the scores; int8: (x + 128) 2^-24, see TreeRows::q_bias.
+template <int KV, bool F16>
+__device__ inline u32x4 tree_widen_k(uint32_t a, uint32_t b) {
+  if constexpr (KV == XLLM_HIP_INT8) {
+    const uint32_t ta = a ^ 0x80808080u, tb = b ^ 0x80808080u;
+    return u32x4{__builtin_amdgcn_perm(0u, ta, 0x0c010c00u), __builtin_amdgcn_perm(0u, ta, 0x0c030c02u),
+                 __builtin_amdgcn_perm(0u, tb, 0x0c010c00u), __builtin_amdgcn_perm(0u, tb, 0x0c030c02u)};
+  } else {
+    return tree_widen<KV, F16>(a, b);
+  }
 }
 
 // Any non-finite value among the 16 bytes?
@@ -284,7 +299,7 @@ struct TreeRows {
   OpK qf[SH::kChunks];
   f32x4 acc[SH::kDT];
   float m_run, l_run;
-  float q_scale;          // kNormQ: factor of the row's scores
+  float q_scale, q_bias;  // int8: the row's scores are s * q_scale + q_bias
   __device__ inline void init(const TreeParams& p, const TreeItem& it, int first_row, int lane) {
     const int kg = lane >> 4;
     const int row = tree_row(p, it, first_row, lane);
@@ -325,6 +340,16 @@ struct TreeRows {
 #pragma unroll
       for (int c = 0; c < SH::kChunks; ++c) qf[c] = __builtin_bit_cast(OpK, raw[c]);
     }
+    if constexpr (SH::kInt8) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int c = 0; c < SH::kChunks; ++c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += (float)qf[c][e];
+      }
+      q_bias = -128.0f * kg_sum(sum) * q_scale;
+      q_scale *= 0x1p24f;
+    }
     m_run = -INFINITY;
     l_run = 0.0f;
 #pragma unroll
@@ -342,7 +367,7 @@ struct TreeRows {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float v = s[i >> 2][i & 3];
-      if constexpr (SH::kNormQ) v *= q_scale;
+      if constexpr (SH::kInt8) v = __builtin_fmaf(v, q_scale, q_bias);
       if constexpr (SH::kQuant) {
         v = __builtin_fmaf(v, kscl[i >> 2][i & 3], lv[i >> 2][i & 3]);
       } else if constexpr (!kFold<MASKED>) {
@@ -523,8 +548,8 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
       for (int h = 0; h < 2; ++h) {
         const u32x4 raw = k_operand(tile, ko, c, h);
         if constexpr (SH::kQuant) {
-          const OpK f0 = __builtin_bit_cast(OpK, tree_widen<KV, SH::kKF16>(raw[0], raw[1]));
-          const OpK f1 = __builtin_bit_cast(OpK, tree_widen<KV, SH::kKF16>(raw[2], raw[3]));
+          const OpK f0 = __builtin_bit_cast(OpK, tree_widen_k<KV, SH::kKF16>(raw[0], raw[1]));
+          const OpK f1 = __builtin_bit_cast(OpK, tree_widen_k<KV, SH::kKF16>(raw[2], raw[3]));
 #pragma unroll
           for (int n = 0; n < N; ++n) {
             s[n][h] = MmaOps<SH::kKF16>::run(f0, rows[a + n].qf[2 * c], s[n][h]);
