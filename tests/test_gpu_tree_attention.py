@@ -192,6 +192,37 @@ def test_long_sequences_are_cut(gpu, kv, n, Hq, Hkv):
         c.check(*c.run(**hints), ref=ref)  # (the last are a captured graph's stale ones)
 
 
+# Hints of a batch so large and ragged that its work is laid on a line and cut into equal pieces, whatever lengths follow.
+ON_A_LINE = dict(max_seq_len=10 ** 6, total_kv_len=6 * 10 ** 6)
+
+
+@pytest.mark.parametrize("q,layout", [("bf16", "HND"), ("fp16", "NHD")])
+@pytest.mark.parametrize("Hq,Hkv,D,bs,most", [(8, 2, 128, 16, 8), (16, 2, 128, 32, 8), (16, 2, 128, 16, 30), (32, 2, 128, 16, 30),
+                                              (14, 2, 64, 32, 4), (14, 2, 64, 32, 8), (28, 2, 64, 16, 20), (4, 2, 256, 16, 8), (24, 3, 256, 64, 15)])
+def test_ragged_batches_in_equal_pieces(gpu, q, layout, Hq, Hkv, D, bs, most):
+    print("case tree line", q, Hq, Hkv, D, bs, most, flush=True)
+    counts = [most, 1, most - 1, 0, 2, most, 3, 1, most // 2]
+    c = TreeCase(counts, [2003, 17, 900, 0, 0, 1300, 3, 1, 288], Hq, Hkv, D, bs, q=q, kv=q, layout=layout, seed=21)
+    ref = c.oracle()
+    out, lse = c.run(**ON_A_LINE)
+    c.check(out, lse, ref=ref)
+    again = c.run(**ON_A_LINE)
+    assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
+def test_ragged_batch_of_many_sequences_in_equal_pieces(gpu):
+    """More sequences than a workgroup has threads, several in a piece, some without rows or tokens; then one alone."""
+    rng = np.random.default_rng(3)
+    lens = rng.integers(0, 40, size=1000)
+    lens[[0, 411, 999]] = (700, 1200, 350)
+    counts = rng.integers(0, 4, size=1000)
+    counts[500:520] = 0
+    c = TreeCase(counts.tolist(), lens, 4, 1, 64, 16, seed=22)
+    c.check(*c.run(max_seq_len=10 ** 6, total_kv_len=6 * 10 ** 8))
+    c = TreeCase([0] * 8 + [2], [5] * 8 + [777], 4, 1, 64, 16, seed=23)
+    c.check(*c.run(**ON_A_LINE))
+
+
 def test_csr_form_uniform_rows_and_strides(gpu):
     c = TreeCase([7, 7, 7], [100, 7, 260], 8, 2, 128, 16, seed=8)
     out, lse = c.run(max_seq_len=300)
@@ -294,10 +325,11 @@ def test_nan_and_infinite_scales_in_unseen_places(gpu):
             scales[blk, :, slot] = keep
 
 
-def test_captured_and_replayed_with_new_lengths(gpu):
+@pytest.mark.parametrize("hints", [{}, dict(max_seq_len=10 ** 6, total_kv_len=18 * 10 ** 5)])
+def test_captured_and_replayed_with_new_lengths(gpu, hints):
     c = TreeCase([9, 9], [900, 700], 16, 4, 128, 16, seed=12)
     lens, out = c.d_lens.clone(), torch.zeros_like(c.q)
-    call = lambda o, n: ops.batch_tree_decode(c.q, c.k, c.v, o, c.d_table, n, c.d_mask, scale=c.scale, q_per_seq=9)  # noqa: E731
+    call = lambda o, n: ops.batch_tree_decode(c.q, c.k, c.v, o, c.d_table, n, c.d_mask, scale=c.scale, q_per_seq=9, **hints)  # noqa: E731
     call(out, lens)
     torch.cuda.synchronize()
     graphs = []

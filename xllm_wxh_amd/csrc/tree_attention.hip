@@ -37,6 +37,11 @@ static int tree_slots(int64_t batch, int64_t n, int64_t hq, int64_t hkv, int64_t
   return s > 1 ? (int)s : 1;
 }
 
+// Where the sequences lie on the line (see TreeLine), for the merge.
+static size_t tree_line_bytes(int64_t batch) {
+  return batch <= kTreeLineBatch ? (size_t)(((batch + 1) * 8 + 255) & ~(int64_t)255) : 0;
+}
+
 static size_t tree_lse_bytes(int64_t batch, int64_t n, int64_t hq, int64_t slots) {
   return (size_t)((batch * slots * n * hq * 4 + 255) & ~(int64_t)255);
 }
@@ -98,13 +103,20 @@ static TreeForm tree_form(const xllm_hip_kv_cache* c, const xllm_hip_decode_args
 //   nearly equal lengths   rounds of equal items:  ceil(items / at_once) * (chunk + kItemTokens)
 //   ragged lengths         the longest chunk while all items run together; else the items' tokens over `at_once`, and
 //                          half a chunk until the last one ends
+//   on a line (TreeLine)   a piece, once more the start of an item, and laying the line
 // plus, where sequences are cut, the merge's launch and the partial results, written once and read once (a row's 4
 // bytes per element against the 2 * eb a cached token takes, shared by the whole GPU).
+// The line serves 16-bit caches: 40 sequences of 800 to 16384 tokens, 8 drafts, 272 -> 246 us; 24 of 800 to 8192, 16
+// drafts, 110 -> 99.  Over 8-bit caches the kernels have no register left for the loop over a piece's items, and what
+// it takes from the loop over the tokens costs more than the even pieces save (100 int8 sequences 217 -> 220 us).
 static void choose_chunks(const xllm_hip_decode_args* a, const TreeForm& form, int eb, TreeParams& p) {
   constexpr int64_t kItemTokens = 128;
   constexpr int64_t kMergeTokens = 128;
+  constexpr int64_t kLineTokens = 64;  // laying the line
   auto whole = [&](int64_t tokens) { return (tokens + p.tile - 1) / p.tile * p.tile; };
   const int64_t longest = a->max_seq_len;
+  const bool can_line = form.rows_per_item > 0 && eb == 2 && p.batch <= kTreeLineBatch && p.slots > 1 && p.num_kv_heads <= form.slots;
+  const int32_t pieces = can_line ? form.slots / p.num_kv_heads : 0;
   if (longest <= 0 || form.rows_per_item == 0) {
     p.chunk = (int32_t)whole(kTreeMinChunk);
     if (longest > 0) {  // (chunk slots no sequence reaches are not launched)
@@ -140,17 +152,36 @@ static void choose_chunks(const xllm_hip_decode_args* a, const TreeForm& form, i
       best_cut = cut;
     }
   }
+  if (can_line) {
+    double t = (double)lanes * (double)(total + p.batch * kItemTokens) / ((double)pieces * p.num_kv_heads);
+    const double least = (double)(longest + kItemTokens) / (double)(p.slots - 1);
+    t = t > least ? t : least;
+    t = (t > kTreeMinChunk ? t : kTreeMinChunk) + kItemTokens + kLineTokens + item_rows * 3.0 / eb + kMergeTokens;
+    if (t < best) {
+      p.pieces = pieces;
+      return;
+    }
+  }
   p.chunk = (int32_t)whole((longest + best_cut - 1) / best_cut);
   p.slots = best_cut;
 }
 
-template <int Q_DT, int COLS>
-static void launch_tree_merge_cols(const TreeParams& p, hipStream_t st) {
+template <int Q_DT, int COLS, bool LINE>
+static void launch_tree_merge_rows(const TreeParams& p, hipStream_t st) {
   const int rows = p.n * p.num_q_heads;  // (p.n <= kTreeMaxNodes)
   if ((int64_t)p.batch * rows <= 8192) {  // two waves to a CU's SIMD
-    tree_merge_kernel<Q_DT, COLS, 1><<<dim3((unsigned)((rows + 3) / 4), (unsigned)p.batch), 256, 0, st>>>(p);
+    tree_merge_kernel<Q_DT, COLS, 1, LINE><<<dim3((unsigned)((rows + 3) / 4), (unsigned)p.batch), 256, 0, st>>>(p);
   } else {
-    tree_merge_kernel<Q_DT, COLS, 4><<<dim3((unsigned)((rows + 15) / 16), (unsigned)p.batch), 256, 0, st>>>(p);
+    tree_merge_kernel<Q_DT, COLS, 4, LINE><<<dim3((unsigned)((rows + 15) / 16), (unsigned)p.batch), 256, 0, st>>>(p);
+  }
+}
+
+template <int Q_DT, int COLS>
+static void launch_tree_merge_cols(const TreeParams& p, hipStream_t st) {
+  if (p.pieces == 0) {
+    launch_tree_merge_rows<Q_DT, COLS, false>(p, st);
+  } else if constexpr (Q_DT != XLLM_HIP_FP32) {
+    launch_tree_merge_rows<Q_DT, COLS, true>(p, st);
   }
 }
 
@@ -165,24 +196,33 @@ static void launch_tree_merge(const TreeParams& p, hipStream_t st) {
   }
 }
 
+template <int QT, int KV, int D, int RTW, int TS, bool STREAM>
+static void launch_tree_mfma_form(const TreeParams& p, unsigned grid, hipStream_t st) {
+  if (p.pieces == 0) {
+    tree_mfma_kernel<QT, KV, D, RTW, TS, STREAM><<<grid, 256, 0, st>>>(p);
+  } else if constexpr (!tree_quant(KV)) {
+    tree_mfma_line_kernel<QT, KV, D, RTW, TS, STREAM><<<grid, 256, 0, st>>>(p);
+  }
+}
+
 template <int QT, int KV, int D>
 static void launch_tree_mfma_d(int rows_per_item, const TreeParams& p, unsigned grid, hipStream_t st) {
   const bool stream = p.row_groups == 1;  // nobody else reads an item's K and V
+  constexpr bool kBoth = tree_quant(KV) && D <= 128;  // (two row tiles of head_dim 256 do not fit the registers)
   if (rows_per_item == 32) {
-    constexpr bool kBoth = tree_quant(KV) && D <= 128;  // (two row tiles of head_dim 256 do not fit the registers)
-    tree_mfma_kernel<QT, KV, D, kBoth ? 2 : 1, kBoth ? 4 : 2, true><<<grid, 256, 0, st>>>(p);
+    launch_tree_mfma_form<QT, KV, D, kBoth ? 2 : 1, kBoth ? 4 : 2, true>(p, grid, st);
   } else if (rows_per_item == 64) {
     if (D < 256 || stream) {
-      tree_mfma_kernel<QT, KV, D, 1, 1, true><<<grid, 256, 0, st>>>(p);
+      launch_tree_mfma_form<QT, KV, D, kBoth ? 2 : 1, kBoth ? 2 : 1, true>(p, grid, st);
     } else {
-      if constexpr (D == 256) tree_mfma_kernel<QT, KV, D, 1, 1, false><<<grid, 256, 0, st>>>(p);
+      if constexpr (D == 256) launch_tree_mfma_form<QT, KV, D, 1, 1, false>(p, grid, st);
     }
   } else {
     if constexpr (D <= 128) {
       if (stream) {
-        tree_mfma_kernel<QT, KV, D, 2, 1, true><<<grid, 256, 0, st>>>(p);
+        launch_tree_mfma_form<QT, KV, D, 2, 1, true>(p, grid, st);
       } else {
-        tree_mfma_kernel<QT, KV, D, 2, 1, false><<<grid, 256, 0, st>>>(p);
+        launch_tree_mfma_form<QT, KV, D, 2, 1, false>(p, grid, st);
       }
     }
   }
@@ -219,7 +259,7 @@ extern "C" size_t xllm_hip_tree_attention_workspace_bytes(int32_t batch, int32_t
   if (batch < 1 || q_per_seq < 1 || num_q_heads < 1 || num_kv_heads < 1 || head_dim < 1) return 0;
   const int64_t s = tree_slots(batch, q_per_seq, num_q_heads, num_kv_heads, head_dim);
   if (s == 1) return 0;
-  return tree_lse_bytes(batch, q_per_seq, num_q_heads, s) + (size_t)(batch * s * q_per_seq * num_q_heads * head_dim * 4);
+  return tree_line_bytes(batch) + tree_lse_bytes(batch, q_per_seq, num_q_heads, s) + (size_t)(batch * s * q_per_seq * num_q_heads * head_dim * 4);
 }
 
 extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
@@ -320,16 +360,20 @@ extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
   const int64_t slots = tree_slots(a->batch, p.n, p.num_q_heads, p.num_kv_heads, p.head_dim);
   p.slots = (int32_t)slots;
   if (slots > 1) {
-    p.partial_lse = (float*)workspace;
-    p.partial_out = (float*)((uint8_t*)workspace + tree_lse_bytes(a->batch, p.n, p.num_q_heads, slots));
+    p.line = (int64_t*)workspace;
+    p.partial_lse = (float*)((uint8_t*)workspace + tree_line_bytes(a->batch));
+    p.partial_out = (float*)((uint8_t*)p.partial_lse + tree_lse_bytes(a->batch, p.n, p.num_q_heads, slots));
   }
   const TreeForm form = tree_form(c, a);
   p.tile = form.rows_per_item > 0 ? 32 : 64;  // (what the kernels take at a time)
   const int64_t rows = (int64_t)p.n * p.group;
   p.row_groups = (int32_t)(form.rows_per_item > 0 ? (rows + form.rows_per_item - 1) / form.rows_per_item : rows);
+  p.rows_per_item = form.rows_per_item;
   choose_chunks(a, form, elem_bytes(c->dtype), p);
   int64_t items = (int64_t)p.batch * p.slots * p.num_kv_heads * p.row_groups;
-  if (form.rows_per_item > 0 && p.row_groups > 1) {  // whole rounds of the XCDs (see the kernel)
+  if (p.pieces > 0) {
+    items = (int64_t)p.pieces * p.num_kv_heads;
+  } else if (form.rows_per_item > 0 && p.row_groups > 1) {  // whole rounds of the XCDs (see the kernel)
     items = (items + kTreeXcds * p.row_groups - 1) / (kTreeXcds * p.row_groups) * (kTreeXcds * p.row_groups);
   }
   XLLM_HIP_REQUIRE(items <= 0x7fffffff, "too many work items: %lld", (long long)items);
@@ -349,7 +393,7 @@ extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
     launch_tree_generic<XLLM_HIP_FP32>(c->dtype, p, grid, st);
   }
   int rc = check_launch("tree attention kernel");
-  if (rc != XLLM_HIP_OK || p.slots == 1) return rc;
+  if (rc != XLLM_HIP_OK || (p.slots == 1 && p.pieces == 0)) return rc;
   if (p.q_dtype == XLLM_HIP_BF16) {
     launch_tree_merge<XLLM_HIP_BF16>(p, st);
   } else if (p.q_dtype == XLLM_HIP_FP16) {

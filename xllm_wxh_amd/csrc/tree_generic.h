@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(64) tree_generic_kernel(TreeParams p) {
 // floats to a lane, D / 4 lanes to a chunk's row (a wave has 64 / (D / 4) chunks' rows at a time), and ROWS query rows
 // to a wave, all of whose loads go out before the first is used: four where there are rows enough, else one, with more
 // of its chunks at a time.
-template <int Q_DT, int COLS, int ROWS>
+template <int Q_DT, int COLS, int ROWS, bool LINE>
 __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
   static_assert(COLS == 16 || COLS == 32 || COLS == 64, "lanes that share a chunk's row, four columns each");
   constexpr int kAtOnce = 64 / COLS;
@@ -105,7 +105,8 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
   const int lane = threadIdx.x & 63;
   // (grid: rows of a sequence, sequences; the workgroups of a sequence that was not cut end here)
   const int b = blockIdx.y;
-  const int chunks = tree_chunks(p, tree_kv_length(p, b));
+  const int len = tree_kv_length(p, b);
+  int chunks = LINE ? 2 : tree_chunks(p, len);
   if (chunks == 1) return;  // written by the attention kernel
   const int per_seq = p.n * p.num_q_heads;
   int64_t q0;
@@ -114,6 +115,28 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
   const int rows = (count < p.n ? count : p.n) * p.num_q_heads;
   const int r0 = ((int)blockIdx.x * 4 + (int)(threadIdx.x >> 6)) * kRows;
   if (r0 >= rows) return;
+  int cut[LINE ? kRows : 1];  // chunks of a row: row groups of one sequence may be cut differently
+  if constexpr (LINE) {
+    const int64_t at = p.line[b], piece = p.line[p.batch];
+    const int units = tree_line_units(len);
+    chunks = 1;
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      cut[k] = 1;
+      if (r0 + k < rows) {
+        const int j = (r0 + k) / p.num_q_heads;
+        const int row = j * p.group + (r0 + k - j * p.num_q_heads) % p.group;
+        cut[k] = tree_line_chunks(at + (int64_t)(row / p.rows_per_item) * units, units, piece);
+      }
+      chunks = cut[k] > chunks ? cut[k] : chunks;
+    }
+    if (chunks == 1) return;
+  }
+  // Chunks to read: none of a row that the attention kernel has written.
+  auto parts = [&](int k) {
+    if constexpr (LINE) return cut[k] > 1 ? cut[k] : 0;
+    return chunks;
+  };
   const int D = p.head_dim;
   const float neg_inf = -INFINITY;
   const int64_t first = (int64_t)b * p.slots * per_seq;  // row r of chunk c: + c * per_seq + r
@@ -129,7 +152,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
       for (int u = 0; u < kUnroll; ++u) {
         const int c = c0 + u * kAtOnce + mine;
         v[k][u] = f32x4{0, 0, 0, 0};
-        if (c < chunks && col < D && r0 + k < rows) {
+        if (c < parts(k) && col < D && r0 + k < rows) {
           const float* src = p.partial_out + (first + (int64_t)c * per_seq + r0 + k) * D + col;
           if (vec) {
             v[k][u] = *(const f32x4*)src;
@@ -144,7 +167,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
   // slots <= 64: a chunk to a lane
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
-    l[k] = lane < chunks && r0 + k < rows ? p.partial_lse[first + (int64_t)lane * per_seq + r0 + k] : neg_inf;
+    l[k] = lane < parts(k) && r0 + k < rows ? p.partial_lse[first + (int64_t)lane * per_seq + r0 + k] : neg_inf;
   }
   load(0);  // (on their way while the weights are formed)
   float e[kRows], m[kRows], total[kRows];
@@ -168,6 +191,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(TreeParams p) {
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
     if (r0 + k >= rows) break;
+    if (LINE && parts(k) == 0) continue;
 #pragma unroll
     for (int s = COLS; s < 64; s <<= 1) {
 #pragma unroll

@@ -15,10 +15,17 @@
 //         lose about a bit.  V has no such end: there the 128 would pile up over the tokens.)
 // With V in fp16 the weights of an 8-bit cache are rounded to 11 bits, those over a bf16 cache to 8.
 //
-// How the waves share an item: 64 rows or 128 rows to a workgroup are 16 or 32 to each wave, which then reads all of
-// the tile.  Up to 32 rows are two tiles of 16: over a 16-bit cache two waves share a row tile, taking alternate 32-token
-// pieces; over an 8-bit cache each wave has both row tiles and every fourth piece, so that a piece is widened once.  The
-// second half of such an item's arithmetic is often unused (16 rows or fewer): a step this narrow is bound by memory.
+// How the waves share an item: 128 rows to a workgroup are 32 to each wave, which then reads all of the tile, and 64 rows
+// over a 16-bit cache 16.  Up to 32 rows are two tiles of 16: over a 16-bit cache two waves share a row tile, taking
+// alternate 32-token pieces.  Over an 8-bit cache every wave has two row tiles, and two (64 rows) or all four (32 rows)
+// share the pieces, because a piece is widened once per wave that takes it (64 x 8192 tokens: int8, 64 rows, 315 -> 258
+// us; 32 rows 225 -> 187; fp8 268 -> 237 and 186 -> 176).  The second half of a narrow item's arithmetic is often unused
+// (16 rows or fewer): a step this narrow is bound by memory.
+//
+// Measured, kernel and merge, bf16 queries, head_dim 128, block_size 16 unless stated:
+//   16-bit cache, 8 or 16 drafts of 4 heads to a kv head, 64 x 4096 or 8192 tokens   164 / 331 us   6.5 TB/s: memory
+//   512 rows to a kv head, 32 x 8192 tokens   bf16 648 us, 850 TFLOP/s; fp8 685 us, 805; int8 770 us, 715: the softmax's
+//   and the widening's vector instructions, which the matrix instructions of one wave only partly cover for another
 //
 // Only the last tokens of a sequence are drafted ones, so only the last pieces are masked.  There a row takes from its
 // mask the 32 bits of the piece; scores of unseen tokens are replaced by -inf whatever they were.  An unseen V may
@@ -458,31 +465,28 @@ struct TreeOut {
 // RTW: row tiles per wave; TS: waves that share the tokens of a set of row tiles, a 32-token piece each in turn; STREAM: see tree_to_lds
 // (one row group; a template argument, because a branch in the loop costs the compiler its schedule: 24 fp8 sequences, 61
 // drafts, 379 against 353 us).
-template <int QT, int KV, int D, int RTW, int TS, bool STREAM>
-__global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1 : 2)) tree_mfma_kernel(TreeParams p) {
+template <int QT, int KV, int D, int RTW, int TS, bool STREAM, bool LINE>
+__device__ __forceinline__ void tree_mfma_item(const TreeParams& p, const TreeItem& it, int wave) {
   typedef TreeShape<QT, KV, D> SH;
-  static_assert(TS == 1 || (TS == 2 && RTW == 1) || TS == 4, "how the end of the item joins the waves' sums");
+  static_assert(TS == 1 || (TS == 2 && RTW == 1) || RTW == 2, "how the end of the item joins the waves' sums");
+  constexpr int kApart = 4 / TS;  // sets of row tiles: wave w has set w % kApart, and share w / kApart of its tokens
   constexpr int kRowsPerItem = 16 * RTW * 4 / TS;
   constexpr int kSums = RTW * SH::kDT * 1024;  // bytes of a wave's accumulators
   __shared__ __attribute__((aligned(16))) uint8_t stage0[SH::kStage];
   __shared__ __attribute__((aligned(16))) uint8_t stage1[SH::kStage];
   __shared__ int found[2][4];  // per stage and wave: a masked tile's V rows hold something that is not finite
-  __shared__ float lds_ml[TS == 4 ? 4 * RTW * 32 : 1];
-  static_assert(TS == 1 || (TS == 2 ? SH::kDT * 1024 + 512 : 2 * kSums) <= SH::kStage, "the exchange of the waves must fit the stages");
+  __shared__ float lds_ml[TS > 1 && RTW == 2 ? 4 * RTW * 32 : 1];
+  static_assert(TS == 1 || (RTW == 1 ? SH::kDT * 1024 + 512 : 2 * kSums) <= SH::kStage, "the exchange of the waves must fit the stages");
 
-  TreeItem it;
-  int id = blockIdx.x;
-  if (p.row_groups > 1) {
-    // the row groups of one (chunk, kv head) read the same K and V: neighbours on one XCD, whose L2 they share
-    const int on = id / kTreeXcds;
-    id = ((on / p.row_groups) * kTreeXcds + id % kTreeXcds) * p.row_groups + on % p.row_groups;
+  int lane = threadIdx.x & 63;
+  if constexpr (LINE) {  // formed anew for every item, like the arguments
+    lane = lane_id();
+    asm volatile("" : "+v"(lane));
+    lane &= 63;
   }
-  if (!tree_item(p, id, kRowsPerItem, it)) return;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
   const int mi = lane & 15, kg = lane >> 4;
-  const int tg = TS == 4 ? wave : TS == 2 ? wave >> 1 : 0;  // which of the waves that share the tokens
-  const int first_row = it.rg * kRowsPerItem + (TS == 4 ? 0 : TS == 2 ? wave & 1 : wave * RTW) * 16;
+  const int tg = wave / kApart;  // which of the waves that share the tokens
+  const int first_row = it.rg * kRowsPerItem + (wave % kApart) * RTW * 16;
 
   TreeLoader<SH, KV> ld;
   ld.init(p, wave, lane);
@@ -734,7 +738,7 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
   // End of the item.  (The lane's number is formed anew: held through the loops it costs a register.)
   const int end_lane = lane_id(), end_kg = end_lane >> 4;
   const float neg_inf = -INFINITY;
-  if constexpr (TS == 2) {
+  if constexpr (TS == 2 && RTW == 1) {
     // the second wave of a row tile hands over its sums; nothing is in flight any more
     __syncthreads();
     uint8_t* xch = (wave & 1) != 0 ? stage1 : stage0;
@@ -760,8 +764,8 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
       r.acc[dt] = r.acc[dt] * a1 + o * a2;
     }
   }
-  if constexpr (TS == 4) {
-    // All four hand over their sums; each finishes a quarter of the head's columns.
+  if constexpr (TS > 1 && RTW == 2) {
+    // All hand over their sums; each finishes its part of the head's columns.
     __syncthreads();
     const int end_mi = end_lane & 15;
     uint8_t* mine = (wave < 2 ? stage0 : stage1) + (wave & 1) * kSums;
@@ -778,24 +782,26 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
     __syncthreads();
 #pragma unroll
     for (int a = 0; a < RTW; ++a) {
-      float m = neg_inf, l = 0.0f, w[4];
+      float m = neg_inf, l = 0.0f, w[TS];
+      const float* ml = lds_ml + ((wave % kApart) * RTW + a) * 32 + end_mi;  // (of share x: + x * kApart * RTW * 32)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) m = fmaxf(m, lds_ml[(x * RTW + a) * 32 + end_mi]);
+      for (int x = 0; x < TS; ++x) m = fmaxf(m, ml[x * kApart * RTW * 32]);
       const float m_safe = m == neg_inf ? 0.0f : m;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        w[x] = __builtin_amdgcn_exp2f(lds_ml[(x * RTW + a) * 32 + end_mi] - m_safe);
-        l += w[x] * lds_ml[(x * RTW + a) * 32 + 16 + end_mi];
+      for (int x = 0; x < TS; ++x) {
+        w[x] = __builtin_amdgcn_exp2f(ml[x * kApart * RTW * 32] - m_safe);
+        l += w[x] * ml[x * kApart * RTW * 32 + 16];
       }
       TreeOut out;
-      if (!out.init(p, it, first_row + 16 * a, end_lane, l, m, wave == 0 && end_kg == 0)) continue;
+      if (!out.init(p, it, first_row + 16 * a, end_lane, l, m, tg == 0 && end_kg == 0)) continue;
 #pragma unroll
-      for (int q = 0; q < SH::kDT / 4; ++q) {
-        const int dt = wave * (SH::kDT / 4) + q;
+      for (int q = 0; q < SH::kDT / TS; ++q) {
+        const int dt = tg * (SH::kDT / TS) + q;
         f32x4 o = {0, 0, 0, 0};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          o += w[x] * *(const f32x4*)((x < 2 ? stage0 : stage1) + (x & 1) * kSums + (a * SH::kDT + dt) * 1024 + end_lane * 16);
+        for (int x = 0; x < TS; ++x) {
+          const int from = x * kApart + wave % kApart;
+          o += w[x] * *(const f32x4*)((from < 2 ? stage0 : stage1) + (from & 1) * kSums + (a * SH::kDT + dt) * 1024 + end_lane * 16);
         }
         out.template store<SH::kQF16>(dt * 16 + 4 * end_kg, o);
       }
@@ -811,6 +817,37 @@ __global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1
     if (!out.init(p, it, first_row + 16 * a, end_lane, l, r.m_run, end_kg == 0)) continue;
 #pragma unroll
     for (int dt = 0; dt < SH::kDT; ++dt) out.template store<SH::kQF16>(dt * 16 + 4 * end_kg, r.acc[dt]);
+  }
+}
+
+template <int QT, int KV, int D, int RTW, int TS, bool STREAM>
+__global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1 : 2)) tree_mfma_kernel(TreeParams p) {
+  TreeItem it;
+  int id = blockIdx.x;
+  if (p.row_groups > 1) {
+    // the row groups of one (chunk, kv head) read the same K and V: neighbours on one XCD, whose L2 they share
+    const int on = id / kTreeXcds;
+    id = ((on / p.row_groups) * kTreeXcds + id % kTreeXcds) * p.row_groups + on % p.row_groups;
+  }
+  if (!tree_item(p, id, 16 * RTW * 4 / TS, it)) return;
+  tree_mfma_item<QT, KV, D, RTW, TS, STREAM, false>(p, it, __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+}
+
+template <int QT, int KV, int D, int RTW, int TS, bool STREAM>
+__global__ void __launch_bounds__(256, (TreeShape<QT, KV, D>::kStage > 40000 ? 1 : 2)) tree_mfma_line_kernel(TreeParams p) {
+  TreeItem it;
+  TreeLine line;
+  if (!line.start(p, blockIdx.x, it)) return;
+  // The arguments are read anew for every item: held in registers from one to the next they are too many.
+  typedef const __attribute__((address_space(4))) TreeParams* Args;
+  Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (;;) {
+    asm volatile("" : "+s"(args));
+    tree_mfma_item<QT, KV, D, RTW, TS, STREAM, true>(*(const TreeParams*)args, it, wave);
+    asm volatile("" : "+s"(args));
+    if (!line.next(*(const TreeParams*)args, it)) return;
+    __syncthreads();  // (nobody reads the stages any more)
   }
 }
 

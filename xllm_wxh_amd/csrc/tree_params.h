@@ -23,6 +23,7 @@ struct TreeParams {
   const uint64_t* mask;
   float* partial_out;  // [batch * slots][n * Hq][head_dim], each row normalised
   float* partial_lse;  // [batch * slots][n * Hq], base 2
+  int64_t* line;       // pieces > 0: where the sequences start on the line, [batch]; behind them the tokens of a piece
   int64_t mask_stride;
   int64_t q_token_stride;
   int64_t out_token_stride;
@@ -48,13 +49,15 @@ struct TreeParams {
   int32_t slots;       // chunks a sequence may have
   int32_t chunk;       // tokens per chunk of a sequence that needs no more than `slots` of them
   int32_t tile;        // chunks are multiples of it
+  int32_t pieces;      // > 0: the work is laid on a line and cut into so many pieces per kv head (see TreeLine)
+  int32_t rows_per_item;
   int32_t q_dtype;
   float scale_log2;    // sm_scale * log2(e)
 };
 
 struct TreeItem {
   int b, hk, rg;
-  int chunk, chunks;   // this item's chunk, chunks of the sequence
+  int chunk, chunks;   // this item's chunk; 1: it is the whole sequence
   int len;             // kv length
   int t_begin, t_end;  // tokens of the chunk
   int prefix;          // tokens every row sees: len - (query tokens of the sequence); may be negative
@@ -103,6 +106,21 @@ __device__ inline void tree_rows(const TreeParams& p, int b, int64_t& q0, int& c
 
 constexpr int kTreeXcds = 8;  // workgroup x runs on XCD x % 8
 
+// The sequence's block list; its length is known.
+__device__ inline void tree_blocks(const TreeParams& p, TreeItem& it) {
+  int64_t listed;
+  if (p.kv_indptr != nullptr) {
+    it.ids = p.block_ids + p.kv_indptr[it.b];
+    listed = (int64_t)p.kv_indptr[it.b + 1] - p.kv_indptr[it.b];
+  } else {
+    it.ids = p.block_ids + (int64_t)it.b * p.bt_stride;
+    listed = p.len_cap / p.block_size;
+  }
+  const int64_t need = ((int64_t)it.len + p.block_size - 1) / p.block_size;
+  it.nblk = (int)(need < listed ? need : listed);
+  if (it.nblk < 1) it.nblk = 1;
+}
+
 // Items in their natural order are (chunk slot, sequence, kv head, row group), row group fastest: the row groups of one
 // (chunk, kv head) read the same K and V, and the sequences' last chunks, which are the short ones, run last.
 __device__ inline bool tree_item(const TreeParams& p, int id, int rows_per_item, TreeItem& it) {
@@ -125,19 +143,139 @@ __device__ inline bool tree_item(const TreeParams& p, int id, int rows_per_item,
   it.t_begin = it.chunk * per;
   const int64_t end = (int64_t)it.t_begin + per;
   it.t_end = end < it.len ? (int)end : it.len;
-  int64_t listed;
-  if (p.kv_indptr != nullptr) {
-    it.ids = p.block_ids + p.kv_indptr[it.b];
-    listed = (int64_t)p.kv_indptr[it.b + 1] - p.kv_indptr[it.b];
-  } else {
-    it.ids = p.block_ids + (int64_t)it.b * p.bt_stride;
-    listed = p.len_cap / p.block_size;
-  }
-  const int64_t need = ((int64_t)it.len + p.block_size - 1) / p.block_size;
-  it.nblk = (int)(need < listed ? need : listed);
-  if (it.nblk < 1) it.nblk = 1;
+  tree_blocks(p, it);
   return true;
 }
+
+// Ragged lengths: the work of a kv head laid on a line, in units of 32 tokens: sequence after sequence, each as often as
+// it has row groups, kTreeStart units for the start of an item and then its tokens.  The line is cut into `pieces` equal
+// pieces, a workgroup each, that run at the same time and end together, whatever the lengths are; a sequence that lies
+// in several pieces leaves a partial in each.  Which piece holds what is computed from the lengths on the device.
+constexpr int kTreeStart = 4;
+constexpr int kTreeLineBatch = 1024;  // sequences: four to a thread that lays the line
+
+__device__ inline int tree_line_groups(const TreeParams& p, int b) {
+  int64_t q0;
+  int count;
+  tree_rows(p, b, q0, count);
+  const int rows = (count < p.n ? count : p.n) * p.group;
+  return (rows + p.rows_per_item - 1) / p.rows_per_item;
+}
+// Units of a sequence; one without tokens has a unit too (its rows are written).
+__device__ inline int tree_line_units(int len) { return kTreeStart + (len > 32 ? (len - 1) / 32 + 1 : 1); }
+
+// Chunks of the row group that starts at `at` on the line: pieces from the one with its first token to the one with its last.
+__device__ inline int tree_line_chunks(int64_t at, int units, int64_t piece) {
+  return (int)((at + units - 1) / piece - (at + kTreeStart) / piece) + 1;
+}
+
+struct TreeLine {
+  int64_t left;  // units of the piece from the start of the current item's sequence on
+
+  // This workgroup's first item; every thread of 256 takes part.  False: there is none.
+  __device__ inline bool start(const TreeParams& p, int id, TreeItem& it) {
+    __shared__ int64_t sums[4];
+    __shared__ int most[4];
+    __shared__ int64_t found[4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    it.hk = id % p.num_kv_heads;
+    const int64_t i = id / p.num_kv_heads;
+    const int per = (p.batch + 255) / 256;
+    int64_t sum = 0;
+    int longest = 0;
+    for (int e = 0; e < per; ++e) {
+      const int b = tid * per + e;
+      if (b >= p.batch) break;
+      const int units = tree_line_units(tree_kv_length(p, b));
+      sum += (int64_t)units * tree_line_groups(p, b);
+      longest = units > longest ? units : longest;
+    }
+    int64_t upto = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t other = __shfl_up(upto, d);
+      if (lane >= d) upto += other;
+      longest = max(longest, __shfl_xor(longest, d));
+    }
+    if (lane == 63) sums[wave] = upto;
+    if (lane == 0) most[wave] = longest;
+    if (tid == 0) found[0] = -1;
+    __syncthreads();
+    int64_t total = 0, at = upto - sum;
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) at += sums[w];
+      total += sums[w];
+      longest = max(longest, most[w]);
+    }
+    // equal pieces; no sequence in more of them than it has slots for partials; none that a partial would outweigh
+    int64_t piece = (int64_t)(((uint64_t)total + (uint32_t)p.pieces - 1) / (uint32_t)p.pieces);
+    const int64_t least = ((int64_t)longest + p.slots - 2) / (p.slots - 1);
+    piece = piece > least ? piece : least;
+    piece = piece > 8 ? piece : 8;
+    piece = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(piece >> 32)) << 32 |
+                      (uint32_t)__builtin_amdgcn_readfirstlane((int)piece));
+    const int64_t from = i * piece;
+    for (int e = 0; e < per; ++e) {
+      const int b = tid * per + e;
+      if (b >= p.batch) break;
+      if (id == 0) p.line[b] = at;
+      const int units = tree_line_units(tree_kv_length(p, b));
+      const int64_t all = (int64_t)units * tree_line_groups(p, b);
+      if (from >= at && from < at + all) {
+        found[1] = (from - at) / units;
+        found[2] = (from - at) % units;
+        found[3] = at;
+        found[0] = b;
+      }
+      at += all;
+    }
+    if (id == 0 && tid == 0) p.line[p.batch] = piece;
+    __syncthreads();
+    it.b = __builtin_amdgcn_readfirstlane((int)found[0]);
+    if (it.b < 0) return false;
+    it.rg = __builtin_amdgcn_readfirstlane((int)found[1]);
+    const int skip = __builtin_amdgcn_readfirstlane((int)found[2]);  // (units of a sequence: below 2^27)
+    sequence(p, it);
+    it.chunk = skip > kTreeStart ? (int)(i - (from - skip + kTreeStart) / piece) : 0;
+    left = piece + skip;
+    it.t_begin = skip > kTreeStart ? (skip - kTreeStart) * 32 : 0;
+    return set_end(it);
+  }
+
+  // The next item of the piece.
+  __device__ inline bool next(const TreeParams& p, TreeItem& it) {
+    left -= tree_line_units(it.len);
+    if (left <= kTreeStart) return false;
+    if ((++it.rg) * p.rows_per_item >= it.n * p.group) {
+      it.rg = 0;
+      do {
+        if (++it.b >= p.batch) return false;
+      } while (tree_line_groups(p, it.b) == 0);
+      sequence(p, it);
+    }
+    it.chunk = 0;
+    it.t_begin = 0;
+    return set_end(it);
+  }
+
+ private:
+  __device__ static inline void sequence(const TreeParams& p, TreeItem& it) {
+    int count;
+    tree_rows(p, it.b, it.q0, count);
+    it.n = count < p.n ? count : p.n;
+    it.len = tree_kv_length(p, it.b);
+    it.prefix = it.len - count;
+    tree_blocks(p, it);
+  }
+  // The item ends with the sequence or with the piece.
+  __device__ inline bool set_end(TreeItem& it) const {
+    const int units = tree_line_units(it.len);
+    const bool whole = left >= units;
+    it.t_end = whole ? it.len : (int)((left - kTreeStart) * 32);
+    it.chunks = whole && it.t_begin == 0 ? 1 : 2;
+    return true;
+  }
+};
 
 // A block id as the kernels use it: within the cache, whatever the table holds.
 __device__ inline int tree_block(const TreeParams& p, int id) {
