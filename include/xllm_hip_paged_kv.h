@@ -630,7 +630,7 @@ int xllm_hip_tree_masks(const int32_t* parents,
  * dealt != 0: in turn, axis(j) = j mod num_axes where j / num_axes < sections[j mod num_axes], else 0.
  * args->positions is [num_axes, num_tokens] with axis_stride elements between the axes; everything else of args,
  * the cache and slot_mapping as in xllm_hip_rope_kv_write (with equal positions on every axis the two calls
- * compute the same).
+ * compute the same formulas; the sum of a head's squares may be formed in another order).
  */
 typedef struct xllm_hip_mrope {
   int32_t num_axes;  /* 1 .. 4 */
@@ -655,7 +655,8 @@ int xllm_hip_mrope_kv_write(const xllm_hip_rope_args* args,
  * lse = -inf.  args as for xllm_hip_paged_decode: either block-list form, q_indptr or q_per_seq, every cache layout
  * and type, lse optional; max_seq_len and total_kv_len are hints that only tune how sequences are cut (0 = unknown).
  * A sliding window (window_left >= 0) and host_plan are refused: XLLM_HIP_UNSUPPORTED.  mask_words <= 8; q_per_seq
- * <= 512 is the largest n_b; tokens past it are ignored.
+ * <= 512 is the largest n_b; tokens past it are ignored.  batch <= 65535.  A quantised cache's V scales must not be
+ * negative (no quantiser makes such), and one below 2^-100 may count as 2^-100 in the weights' sum of products.
  * `workspace` (256-byte aligned, xllm_hip_tree_attention_workspace_bytes) holds the partial results of sequences that
  * were cut: written and read within the call, nothing is kept from one call to the next.  One call at a time may
  * use it.

@@ -462,9 +462,9 @@ struct TreeOut {
   }
 };
 
-// RTW: row tiles per wave; TS: waves that share the tokens of a set of row tiles, a 32-token piece each in turn; STREAM: see tree_to_lds
-// (one row group; a template argument, because a branch in the loop costs the compiler its schedule: 24 fp8 sequences, 61
-// drafts, 379 against 353 us).
+// RTW: row tiles per wave; TS: waves that share the tokens of a set of row tiles, a 32-token piece each in turn; STREAM:
+// see tree_to_lds (one row group; a template argument, because a branch in the loop costs the compiler its schedule: 24
+// fp8 sequences, 61 drafts, 379 against 353 us); LINE: the item is one of several of its workgroup.
 template <int QT, int KV, int D, int RTW, int TS, bool STREAM, bool LINE>
 __device__ __forceinline__ void tree_mfma_item(const TreeParams& p, const TreeItem& it, int wave) {
   typedef TreeShape<QT, KV, D> SH;
