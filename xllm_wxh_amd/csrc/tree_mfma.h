@@ -582,7 +582,9 @@ __device__ __forceinline__ void tree_mfma_item(const TreeParams& p, const TreeIt
     constexpr bool MASKED = decltype(masked)::value;
     const uint8_t* tile = stage + piece * SH::kRB;
     f32x4 s[RTW][2];
+    __builtin_amdgcn_s_setprio(1);  // matrix instructions before the other workgroup's softmax (fp8, 512 rows: 2 %)
     scores(tile, std::integral_constant<int, RTW>{}, 0, s);
+    __builtin_amdgcn_s_setprio(0);
     uint32_t vis[RTW];
 #pragma unroll
     for (int a = 0; a < RTW; ++a) vis[a] = MASKED ? masks[a].bits(p, it, first_row + 16 * a, lane, tb + piece) : 0u;
@@ -622,6 +624,7 @@ __device__ __forceinline__ void tree_mfma_item(const TreeParams& p, const TreeIt
         for (int dt = 0; dt < SH::kDT; ++dt) rows[a].acc[dt] *= alpha[a];
       }
     }
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int dt = 0; dt < SH::kDT; ++dt) {
       OpV vf;
@@ -633,6 +636,7 @@ __device__ __forceinline__ void tree_mfma_item(const TreeParams& p, const TreeIt
 #pragma unroll
       for (int a = 0; a < RTW; ++a) rows[a].acc[dt] = MmaOps<SH::kVF16>::run(vf, pf[a], rows[a].acc[dt]);
     }
+    __builtin_amdgcn_s_setprio(0);
   };
 
   // The same where V holds something that is not finite: token by token, each row under its own bits, a row tile after
