@@ -67,7 +67,7 @@ def run_indices(dev, cached, new, block_size, pool, *, request_ids=None, held=No
 
 
 @pytest.mark.parametrize("block_size", [1, 16, 24, 128])
-@pytest.mark.parametrize("B,top", [(1, 1), (7, 40), (300, 9), (1100, 5)])
+@pytest.mark.parametrize("B,top", [(1, 1), (7, 40), (300, 9), (512, 3), (513, 3), (1100, 5), (4096, 2)])
 def test_step_indices_with_allocation(gpu, B, top, block_size):
     print("case indices", B, top, block_size, flush=True)
     rng = np.random.default_rng(B + block_size)

@@ -6,7 +6,7 @@
 // Both are launch-bound: the arrays of a decode step are kilobytes, those of a large mixed step a megabyte.  So
 // each is one launch in which no workgroup waits for another: a workgroup that needs sums over the sequences in
 // front of its own forms them itself from the lengths (4096 sequences at most: 48 KiB, from L2).  8 sequences of 4096
-// tokens, one new token each: 4.8 us; 255 sequences of up to 9001 tokens and 700 new ones: 8.4, the loads of the
+// tokens, one new token each: 4.8 us; 255 sequences of up to 9001 tokens and 700 new ones: 7.8, the loads of the
 // lengths, the scan, the search for a row's sequence and the load of its block one after another.
 #include "device_utils.h"
 #include "host_utils.h"
@@ -93,6 +93,7 @@ __device__ inline void table_part(const StepParams& p, int wg, int64_t* lds) {
   const int tid = threadIdx.x;
   int64_t tokens = 0, grown = 0, listed = 0, taken = 0, missing = 0;
   const int64_t head = free_start(p);
+  SeqNeed next = b0 < a.batch ? seq_need(p, b0) : SeqNeed{};  // (on its way while the sums are formed)
   for (int b = tid; b < b0; b += kStepThreads) {
     const SeqNeed s = seq_need(p, b);
     tokens += s.n;
@@ -116,7 +117,8 @@ __device__ inline void table_part(const StepParams& p, int wg, int64_t* lds) {
   }
   const int b1 = b0 + p.seqs_per_wg < a.batch ? b0 + p.seqs_per_wg : a.batch;
   for (int b = b0; b < b1; ++b) {
-    const SeqNeed s = seq_need(p, b);
+    const SeqNeed s = next;
+    if (b + 1 < b1) next = seq_need(p, b + 1);
     const int64_t first = head + grown;
     const int avail = blocks_available(p, s, first);
     const int rows = s.need < a.table_width ? (int)s.need : a.table_width;  // listed blocks
@@ -169,8 +171,23 @@ __device__ inline void table_part(const StepParams& p, int wg, int64_t* lds) {
   }
 }
 
+// What the token rows need of the sequences: exclusive sums of token counts and of blocks taken; up to 512 sequences
+// also what seq_need fetched, so that a row does not wait for it again (255 sequences 8.7 -> 7.8 us; the 96 KiB of 4096
+// sequences would leave a CU one workgroup: 2000 sequences 16.9 -> 22.5).
+template <int N>
+struct StepSums {
+  static constexpr bool kKept = N <= 512;
+  int32_t q[N + 1];
+  int32_t grow[N];
+  int32_t cached[kKept ? N : 1];
+  int32_t held[kKept ? N : 1];
+  int32_t row[kKept ? N : 1];
+  int32_t avail[kKept ? N : 1];
+};
+
 // Slots and positions of kStepTile token rows.
-__device__ inline void token_part(const StepParams& p, int wg, int32_t* q_off, int32_t* grow_off, int64_t* lds) {
+template <int N>
+__device__ inline void token_part(const StepParams& p, int wg, StepSums<N>& of, int64_t* lds) {
   const xllm_hip_step_args& a = p.a;
   const int tid = threadIdx.x;
   const int wave = tid >> 6, lane = tid & 63;
@@ -203,18 +220,24 @@ __device__ inline void token_part(const StepParams& p, int wg, int32_t* q_off, i
     nb += lds[2 * w];
     gb += lds[2 * w + 1];
   }
+  const int64_t head = free_start(p);
   for (int b = s0; b < s1; ++b) {
     const SeqNeed s = seq_need(p, b);
-    q_off[b] = clip32(nb);
-    grow_off[b] = clip32(gb);
+    of.q[b] = clip32(nb);
+    of.grow[b] = clip32(gb);
+    if constexpr (StepSums<N>::kKept) {
+      of.cached[b] = (int32_t)s.cached;
+      of.held[b] = s.held;
+      of.row[b] = s.row;
+      of.avail[b] = blocks_available(p, s, head + gb);
+    }
     nb += s.n;
     gb += s.grow;
-    if (b == a.batch - 1) q_off[a.batch] = clip32(nb);
+    if (b == a.batch - 1) of.q[a.batch] = clip32(nb);
   }
-  if (a.batch == 0 && tid == 0) q_off[0] = 0;
+  if (a.batch == 0 && tid == 0) of.q[0] = 0;
   __syncthreads();
-  const int64_t total = q_off[a.batch];
-  const int64_t head = free_start(p);
+  const int64_t total = of.q[a.batch];
 #pragma unroll
   for (int u = 0; u < kStepTile / kStepThreads; ++u) {
     const int64_t t = (int64_t)wg * kStepTile + u * kStepThreads + tid;
@@ -224,17 +247,27 @@ __device__ inline void token_part(const StepParams& p, int wg, int32_t* q_off, i
       int lo = 0, hi = a.batch;  // the last sequence whose offset is <= t (behind empty ones)
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (q_off[mid] <= t) {
+        if (of.q[mid] <= t) {
           lo = mid;
         } else {
           hi = mid;
         }
       }
-      const SeqNeed s = seq_need(p, lo);
-      const int64_t first = head + grow_off[lo];
-      pos = s.cached + (t - q_off[lo]);
+      const int64_t first = head + of.grow[lo];
+      SeqNeed s;
+      int avail;
+      if constexpr (StepSums<N>::kKept) {
+        s.cached = of.cached[lo];
+        s.held = of.held[lo];
+        s.row = of.row[lo];
+        avail = of.avail[lo];
+      } else {
+        s = seq_need(p, lo);
+        avail = blocks_available(p, s, first);
+      }
+      pos = s.cached + (t - of.q[lo]);
       const int64_t i = p.log2_bs >= 0 ? pos >> p.log2_bs : pos / a.block_size;
-      if (i < blocks_available(p, s, first)) {
+      if (i < avail) {
         const int id = block_id(p, s, (int)i, first);
         slot = (int64_t)id * a.block_size + (pos - i * a.block_size);
         if (id < 0 || slot > INT_MAX) slot = -1;
@@ -249,14 +282,15 @@ __device__ inline void token_part(const StepParams& p, int wg, int32_t* q_off, i
   }
 }
 
+// N: sequences at most.
+template <int N>
 __global__ void __launch_bounds__(kStepThreads) step_indices_kernel(StepParams p) {
-  __shared__ int32_t q_off[kStepMaxBatch + 1];
-  __shared__ int32_t grow_off[kStepMaxBatch];
+  __shared__ StepSums<N> sums;
   __shared__ int64_t lds[12];
   if ((int)blockIdx.x < p.table_wgs) {
     table_part(p, blockIdx.x, lds);
   } else {
-    token_part(p, blockIdx.x - p.table_wgs, q_off, grow_off, lds);
+    token_part(p, blockIdx.x - p.table_wgs, sums, lds);
   }
 }
 
@@ -414,7 +448,12 @@ extern "C" int xllm_hip_build_step_indices(const xllm_hip_step_args* a, xllm_hip
   const int64_t token_wgs = (a->num_rows + kStepTile - 1) / kStepTile;
   XLLM_HIP_REQUIRE(table_wgs + token_wgs <= 0x7fffffff, "too many rows");
   p.table_wgs = (int32_t)table_wgs;
-  step_indices_kernel<<<(unsigned)(table_wgs + token_wgs), kStepThreads, 0, (hipStream_t)stream>>>(p);
+  const unsigned grid = (unsigned)(table_wgs + token_wgs);
+  if (a->batch <= 512) {
+    step_indices_kernel<512><<<grid, kStepThreads, 0, (hipStream_t)stream>>>(p);
+  } else {
+    step_indices_kernel<kStepMaxBatch><<<grid, kStepThreads, 0, (hipStream_t)stream>>>(p);
+  }
   return check_launch("step_indices_kernel");
 }
 
