@@ -325,11 +325,10 @@ def test_nan_and_infinite_scales_in_unseen_places(gpu):
             scales[blk, :, slot] = keep
 
 
-@pytest.mark.parametrize("hints", [{}, dict(max_seq_len=10 ** 6, total_kv_len=18 * 10 ** 5)])
-def test_captured_and_replayed_with_new_lengths(gpu, hints):
+def test_captured_and_replayed_with_new_lengths(gpu):
     c = TreeCase([9, 9], [900, 700], 16, 4, 128, 16, seed=12)
     lens, out = c.d_lens.clone(), torch.zeros_like(c.q)
-    call = lambda o, n: ops.batch_tree_decode(c.q, c.k, c.v, o, c.d_table, n, c.d_mask, scale=c.scale, q_per_seq=9, **hints)  # noqa: E731
+    call = lambda o, n: ops.batch_tree_decode(c.q, c.k, c.v, o, c.d_table, n, c.d_mask, scale=c.scale, q_per_seq=9)  # noqa: E731
     call(out, lens)
     torch.cuda.synchronize()
     graphs = []
@@ -347,6 +346,29 @@ def test_captured_and_replayed_with_new_lengths(gpu, hints):
             g.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want), (a, b)
+
+
+def test_equal_pieces_captured_and_replayed_with_new_lengths(gpu):
+    top = [900, 700, 9, 2100, 40, 333, 1200, 64, 500]
+    c = TreeCase([9] * 9, top, 16, 2, 128, 16, seed=24)
+    lens, out = c.d_lens.clone(), torch.zeros_like(c.q)
+    call = lambda o: ops.batch_tree_decode(c.q, c.k, c.v, o, c.d_table, lens, c.d_mask, scale=c.scale, q_per_seq=9, **ON_A_LINE)  # noqa: E731
+    call(out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(out)
+    for step in range(4):
+        now = [max(9, n // (step + 1) - step) if (b + step) % 3 else 9 for b, n in enumerate(top)]
+        lens.copy_(torch.tensor(now, dtype=torch.int32, device=gpu))
+        want = torch.empty_like(out)
+        call(want)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), now
+        c.lens = np.asarray(now, np.int32)
+        c.check(want, c.run(lens=lens, **ON_A_LINE)[1])
 
 
 def test_two_streams_at_once(gpu):

@@ -97,26 +97,22 @@ static TreeForm tree_form(const xllm_hip_kv_cache* c, const xllm_hip_decode_args
   return f;
 }
 
-// Tokens per chunk and chunks per sequence (at most p.slots of them on entry).  Without the host's lengths: as many
-// chunks as the workspace holds, of at least kTreeMinChunk tokens.  With them, the cut whose step is predicted to end
-// first, counted in tokens a workgroup gets through (`at_once` of them run together):
-//   nearly equal lengths   rounds of equal items:  ceil(items / at_once) * (chunk + kItemTokens)
-//   ragged lengths         the longest chunk while all items run together; else the items' tokens over `at_once`, and
+// Tokens per chunk and chunks per sequence (at most p.slots of them on entry), or pieces of a line.  Without the host's
+// lengths: as many chunks as the workspace holds, of at least kTreeMinChunk tokens.  With them, the cut whose step is
+// predicted to end first, from what a token costs where all workgroups run (`slots` of them): its K and V at the memory's
+// rate, or its products at that of the matrix kernels, whichever is more,
+//   nearly equal lengths   rounds of equal items:  ceil(items / slots) * (chunk + start)
+//   ragged lengths         the longest chunk while all items run together; else the items' tokens over `slots`, and
 //                          half a chunk until the last one ends
-//   on a line (TreeLine)   a piece, once more the start of an item, and laying the line
-// plus, where sequences are cut, the merge's launch and the partial results, written once and read once (a row's 4
-// bytes per element against the 2 * eb a cached token takes, shared by the whole GPU).
+//   on a line (TreeLine)   a piece, one more start, and laying the line
+// plus, where sequences are cut, the merge's launch and the partial results, written once and read once.
 // The line serves 16-bit caches: 40 sequences of 800 to 16384 tokens, 8 drafts, 272 -> 246 us; 24 of 800 to 8192, 16
-// drafts, 110 -> 99.  Over 8-bit caches the kernels have no register left for the loop over a piece's items, and what
-// it takes from the loop over the tokens costs more than the even pieces save (100 int8 sequences 217 -> 220 us).
+// drafts, 110 -> 99; 103 of up to 2208, 31 drafts, head_dim 256, 263 -> 198.  Over 8-bit caches the kernels have no
+// register left for the loop over a piece's items, and what it takes from the loop over the tokens costs more than the
+// even pieces save (100 int8 sequences 217 -> 220 us).
 static void choose_chunks(const xllm_hip_decode_args* a, const TreeForm& form, int eb, TreeParams& p) {
-  constexpr int64_t kItemTokens = 128;
-  constexpr int64_t kMergeTokens = 128;
-  constexpr int64_t kLineTokens = 64;  // laying the line
   auto whole = [&](int64_t tokens) { return (tokens + p.tile - 1) / p.tile * p.tile; };
   const int64_t longest = a->max_seq_len;
-  const bool can_line = form.rows_per_item > 0 && eb == 2 && p.batch <= kTreeLineBatch && p.slots > 1 && p.num_kv_heads <= form.slots;
-  const int32_t pieces = can_line ? form.slots / p.num_kv_heads : 0;
   if (longest <= 0 || form.rows_per_item == 0) {
     p.chunk = (int32_t)whole(kTreeMinChunk);
     if (longest > 0) {  // (chunk slots no sequence reaches are not launched)
@@ -128,35 +124,40 @@ static void choose_chunks(const xllm_hip_decode_args* a, const TreeForm& form, i
   int64_t total = a->total_kv_len;
   if (total <= 0 || total > longest * p.batch) total = longest * p.batch;
   const bool equal = longest * p.batch * 4 <= total * 5;
-  const int64_t lanes = (int64_t)p.num_kv_heads * p.row_groups;
-  const int64_t item_rows = (int64_t)p.n * p.group < form.rows_per_item ? (int64_t)p.n * p.group : form.rows_per_item;
+  const double lanes = (double)p.num_kv_heads * p.row_groups;
+  const double rows = (double)p.n * p.group < form.rows_per_item ? (double)p.n * p.group : (double)form.rows_per_item;
+  // ns (6.5 bytes, 850 kflop in one)
+  const double bytes = 2.0 * p.head_dim * eb * form.slots / 6.5e3;
+  const double flops = 4.0 * p.head_dim * form.rows_per_item * form.slots / 850e3;
+  const double token = bytes > flops ? bytes : flops;
+  const double partial = rows * 8.0 * p.head_dim / 6.5e3;
+  constexpr double kStart = 5000.0, kMerge = 5000.0, kLine = 5000.0;
   double best = 0.0;
   int best_cut = 0;
   for (int cut = 1; cut <= p.slots; ++cut) {
     const int64_t chunk = whole((longest + cut - 1) / cut);
     if (cut > 1 && chunk < kTreeMinChunk) break;
-    double t;
+    const double item = (double)chunk * token + kStart;
+    double items, t;
     if (equal) {
-      const int64_t items = lanes * p.batch * ((longest + chunk - 1) / chunk);
-      t = (double)((items + form.slots - 1) / form.slots) * (double)(chunk + kItemTokens);
-      if (cut > 1) t += (double)items * item_rows * 2.0 / eb / form.slots;
+      items = lanes * p.batch * (double)((longest + chunk - 1) / chunk);
+      t = ceil(items / form.slots) * item;
     } else {
-      const double items = (double)lanes * ((double)total / (double)chunk + 0.5 * p.batch);
-      t = items <= (double)form.slots ? (double)(chunk + kItemTokens)
-                                      : ((double)lanes * (double)total + items * kItemTokens) / form.slots + 0.5 * (double)chunk;
-      if (cut > 1) t += items * item_rows * 2.0 / eb / form.slots;
+      items = lanes * ((double)total / (double)chunk + 0.5 * p.batch);
+      t = items <= (double)form.slots ? item : (lanes * (double)total * token + items * kStart) / form.slots + 0.5 * (double)chunk * token;
     }
-    if (cut > 1) t += kMergeTokens;
+    if (cut > 1) t += items * partial + kMerge;
     if (best_cut == 0 || t < best) {
       best = t;
       best_cut = cut;
     }
   }
-  if (can_line) {
-    double t = (double)lanes * (double)(total + p.batch * kItemTokens) / ((double)pieces * p.num_kv_heads);
-    const double least = (double)(longest + kItemTokens) / (double)(p.slots - 1);
-    t = t > least ? t : least;
-    t = (t > kTreeMinChunk ? t : kTreeMinChunk) + kItemTokens + kLineTokens + item_rows * 3.0 / eb + kMergeTokens;
+  if (eb == 2 && p.batch <= kTreeLineBatch && p.slots > 1 && p.num_kv_heads <= form.slots) {
+    const int32_t pieces = form.slots / p.num_kv_heads;
+    const double wgs = (double)pieces * p.num_kv_heads;
+    double t = lanes * ((double)total * token + p.batch * kStart) / wgs;
+    const double least = (double)longest / (double)(p.slots - 1), piece = (least > kTreeMinChunk ? least : (double)kTreeMinChunk) * token;
+    t = (t > piece ? t : piece) + kStart + kLine + 1.5 * wgs * partial + kMerge;
     if (t < best) {
       p.pieces = pieces;
       return;
