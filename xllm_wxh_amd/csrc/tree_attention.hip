@@ -98,9 +98,12 @@ static TreeForm tree_form(const xllm_hip_kv_cache* c, const xllm_hip_decode_args
 }
 
 // Tokens per chunk and chunks per sequence (at most p.slots of them on entry), or pieces of a line.  Without the host's
-// lengths: as many chunks as the workspace holds, of at least kTreeMinChunk tokens.  With them, the cut whose step is
-// predicted to end first, from what a token costs where all workgroups run (`slots` of them): its K and V at the memory's
-// rate, or its products at that of the matrix kernels, whichever is more,
+// lengths: from 64 (sequence, kv head, row group)s on the line where it serves (64 x 4096 bf16 tokens, 8 drafts: 170 us
+// against 208 in chunks; 2 x 700 tokens, 16 of them, 16 against 12), else chunks of at least
+// kTreeMinChunk tokens, as many to a sequence as make 1024 items (with 2048, 32 x 8192 fp8 tokens and 512 query rows to a
+// kv head take 848 us against 673).  With them, the cut whose step is predicted to end first, from what a token costs
+// where all workgroups run (`slots` of them): its K and V at the memory's rate, or its products at that of the matrix
+// kernels, whichever is more,
 //   nearly equal lengths   rounds of equal items:  ceil(items / slots) * (chunk + start)
 //   ragged lengths         the longest chunk while all items run together; else the items' tokens over `slots`, and
 //                          half a chunk until the last one ends
@@ -113,8 +116,18 @@ static TreeForm tree_form(const xllm_hip_kv_cache* c, const xllm_hip_decode_args
 static void choose_chunks(const xllm_hip_decode_args* a, const TreeForm& form, int eb, TreeParams& p) {
   auto whole = [&](int64_t tokens) { return (tokens + p.tile - 1) / p.tile * p.tile; };
   const int64_t longest = a->max_seq_len;
+  const bool can_line = form.rows_per_item > 0 && eb == 2 && p.batch <= kTreeLineBatch && p.slots > 1 && p.num_kv_heads <= form.slots;
+  const int32_t pieces = can_line ? form.slots / p.num_kv_heads : 0;
+  if (longest <= 0 && can_line && (int64_t)p.batch * p.num_kv_heads * p.row_groups >= 64) {
+    p.pieces = pieces;
+    return;
+  }
   if (longest <= 0 || form.rows_per_item == 0) {
     p.chunk = (int32_t)whole(kTreeMinChunk);
+    if (longest <= 0 && form.rows_per_item > 0) {
+      const int64_t lanes = (int64_t)p.batch * p.num_kv_heads * p.row_groups, cuts = (1024 + lanes - 1) / lanes;
+      if (cuts < p.slots) p.slots = (int32_t)cuts;
+    }
     if (longest > 0) {  // (chunk slots no sequence reaches are not launched)
       const int64_t most = (longest + p.chunk - 1) / p.chunk;
       if (most < p.slots) p.slots = (int32_t)most;
@@ -152,8 +165,7 @@ static void choose_chunks(const xllm_hip_decode_args* a, const TreeForm& form, i
       best_cut = cut;
     }
   }
-  if (eb == 2 && p.batch <= kTreeLineBatch && p.slots > 1 && p.num_kv_heads <= form.slots) {
-    const int32_t pieces = form.slots / p.num_kv_heads;
+  if (can_line) {
     const double wgs = (double)pieces * p.num_kv_heads;
     double t = lanes * ((double)total * token + p.batch * kStart) / wgs;
     const double least = (double)longest / (double)(p.slots - 1), piece = (least > kTreeMinChunk ? least : (double)kTreeMinChunk) * token;
