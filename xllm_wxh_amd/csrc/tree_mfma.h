@@ -24,7 +24,7 @@
 //
 // Measured, kernel and merge, bf16 queries, head_dim 128, block_size 16 unless stated:
 //   16-bit cache, 8 or 16 drafts of 4 heads to a kv head, 64 x 4096 or 8192 tokens   164 / 331 us   6.5 TB/s: memory
-//   512 rows to a kv head, 32 x 8192 tokens   bf16 648 us, 850 TFLOP/s; fp8 685 us, 805; int8 770 us, 715: the softmax's
+//   512 rows to a kv head, 32 x 8192 tokens   bf16 648 us, 850 TFLOP/s; fp8 662 us, 830; int8 770 us, 715: the softmax's
 //   and the widening's vector instructions, which the matrix instructions of one wave only partly cover for another
 //
 // Only the last tokens of a sequence are drafted ones, so only the last pieces are masked.  There a row takes from its
@@ -485,8 +485,9 @@ __device__ __forceinline__ void tree_mfma_item(const TreeParams& p, const TreeIt
     lane &= 63;
   }
   const int mi = lane & 15, kg = lane >> 4;
-  const int tg = wave / kApart;  // which of the waves that share the tokens
-  const int first_row = it.rg * kRowsPerItem + (wave % kApart) * RTW * 16;
+  // (TS == 1 spelled out: the compiler does not know that there are four waves; fp8, 512 rows, 670 against 662 us)
+  const int tg = TS == 1 ? 0 : wave / kApart;  // which of the waves that share the tokens
+  const int first_row = it.rg * kRowsPerItem + (TS == 1 ? wave : wave % kApart) * RTW * 16;
 
   TreeLoader<SH, KV> ld;
   ld.init(p, wave, lane);
@@ -582,9 +583,12 @@ __device__ __forceinline__ void tree_mfma_item(const TreeParams& p, const TreeIt
     constexpr bool MASKED = decltype(masked)::value;
     const uint8_t* tile = stage + piece * SH::kRB;
     f32x4 s[RTW][2];
-    __builtin_amdgcn_s_setprio(1);  // matrix instructions before the other workgroup's softmax (fp8, 512 rows: 2 %)
+    // Matrix instructions before the other workgroup's softmax: fp8, 512 rows to a kv head, 2 % faster.  (The forms that
+    // are bound by memory or latency lose half a microsecond to what it does to their schedule.)
+    constexpr bool kFirst = SH::kQuant || RTW > 1;
+    if constexpr (kFirst) __builtin_amdgcn_s_setprio(1);
     scores(tile, std::integral_constant<int, RTW>{}, 0, s);
-    __builtin_amdgcn_s_setprio(0);
+    if constexpr (kFirst) __builtin_amdgcn_s_setprio(0);
     uint32_t vis[RTW];
 #pragma unroll
     for (int a = 0; a < RTW; ++a) vis[a] = MASKED ? masks[a].bits(p, it, first_row + 16 * a, lane, tb + piece) : 0u;
@@ -624,7 +628,7 @@ __device__ __forceinline__ void tree_mfma_item(const TreeParams& p, const TreeIt
         for (int dt = 0; dt < SH::kDT; ++dt) rows[a].acc[dt] *= alpha[a];
       }
     }
-    __builtin_amdgcn_s_setprio(1);
+    if constexpr (kFirst) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int dt = 0; dt < SH::kDT; ++dt) {
       OpV vf;
@@ -636,7 +640,7 @@ __device__ __forceinline__ void tree_mfma_item(const TreeParams& p, const TreeIt
 #pragma unroll
       for (int a = 0; a < RTW; ++a) rows[a].acc[dt] = MmaOps<SH::kVF16>::run(vf, pf[a], rows[a].acc[dt]);
     }
-    __builtin_amdgcn_s_setprio(0);
+    if constexpr (kFirst) __builtin_amdgcn_s_setprio(0);
   };
 
   // The same where V holds something that is not finite: token by token, each row under its own bits, a row tile after
