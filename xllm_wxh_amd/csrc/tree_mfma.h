@@ -607,10 +607,11 @@ __device__ __forceinline__ void tree_mfma_item(const TreeParams& p, const TreeIt
     f32x4 rvs[2];
     factor(stage, piece, 2, rvs);
     const uint32_t vo = fresh(v_off);
+    constexpr int kFetched = SH::kNormQ && TS == 1 ? SH::kDT - 1 : SH::kDT;  // (all of them would spill)
     i32x2 vraw[kAhead ? SH::kDT : 1];
     if constexpr (kAhead) {
 #pragma unroll
-      for (int dt = 0; dt < SH::kDT; ++dt) vraw[dt] = v_bytes(tile, vo, dt);
+      for (int dt = 0; dt < kFetched; ++dt) vraw[dt] = v_bytes(tile, vo, dt);
       __builtin_amdgcn_sched_barrier(0);
     }
     OpV pf[RTW];
@@ -632,7 +633,7 @@ __device__ __forceinline__ void tree_mfma_item(const TreeParams& p, const TreeIt
 #pragma unroll
     for (int dt = 0; dt < SH::kDT; ++dt) {
       OpV vf;
-      if constexpr (kAhead) {
+      if (kAhead && dt < kFetched) {
         vf = __builtin_bit_cast(OpV, tree_widen<KV, SH::kVF16>((uint32_t)vraw[dt][0], (uint32_t)vraw[dt][1]));
       } else {
         vf = v_operand(tile, vo, dt);
