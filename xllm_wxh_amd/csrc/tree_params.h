@@ -176,7 +176,7 @@ struct TreeLine {
   __device__ inline bool start(const TreeParams& p, int id, TreeItem& it) {
     __shared__ int64_t sums[4];
     __shared__ int most[4];
-    __shared__ int64_t found[4];
+    __shared__ int64_t found[3];  // the sequence, its row group and the units of it before the piece
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     it.hk = id % p.num_kv_heads;
     const int64_t i = id / p.num_kv_heads;
@@ -224,7 +224,6 @@ struct TreeLine {
       if (from >= at && from < at + all) {
         found[1] = (from - at) / units;
         found[2] = (from - at) % units;
-        found[3] = at;
         found[0] = b;
       }
       at += all;
@@ -239,7 +238,8 @@ struct TreeLine {
     it.chunk = skip > kTreeStart ? (int)(i - (from - skip + kTreeStart) / piece) : 0;
     left = piece + skip;
     it.t_begin = skip > kTreeStart ? (skip - kTreeStart) * 32 : 0;
-    return set_end(it);
+    set_end(it);
+    return true;
   }
 
   // The next item of the piece.
@@ -255,7 +255,8 @@ struct TreeLine {
     }
     it.chunk = 0;
     it.t_begin = 0;
-    return set_end(it);
+    set_end(it);
+    return true;
   }
 
  private:
@@ -268,12 +269,11 @@ struct TreeLine {
     tree_blocks(p, it);
   }
   // The item ends with the sequence or with the piece.
-  __device__ inline bool set_end(TreeItem& it) const {
+  __device__ inline void set_end(TreeItem& it) const {
     const int units = tree_line_units(it.len);
     const bool whole = left >= units;
     it.t_end = whole ? it.len : (int)((left - kTreeStart) * 32);
     it.chunks = whole && it.t_begin == 0 ? 1 : 2;
-    return true;
   }
 };
 
