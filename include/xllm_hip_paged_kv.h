@@ -675,6 +675,19 @@ int xllm_hip_tree_attention(const xllm_hip_kv_cache* cache,
                             size_t workspace_bytes,
                             xllm_hip_stream_t stream);
 
+/* How xllm_hip_tree_attention would run these arguments: host-only, launches nothing, reads no device memory.  It exists so
+ * that the choice of kernel and cut can be inspected, and tested, without a GPU.  Writes up to `count` of
+ *   out[0]  query rows per workgroup of the matrix kernels, 0: the generic kernel
+ *   out[1]  workgroups of the attention launch
+ *   out[2]  row groups a (sequence, kv head)'s query rows are cut into
+ *   out[3]  equal pieces of the line per kv head, 0: sequences are cut into chunks
+ *   out[4]  tokens per chunk (0 on the line)            out[5]  chunks (partial results) a sequence may have
+ * zeros behind them and for an empty batch; returns XLLM_HIP_OK, or the error the same arguments would get. */
+int xllm_hip_tree_attention_describe(const xllm_hip_kv_cache* cache,
+                                     const xllm_hip_decode_args* args,
+                                     int64_t* out,
+                                     int32_t count);
+
 /*
  * The cache rows of the accepted path moved to the front of the drafted range, for one layer's cache: with
  * c = cached_lens[b] (the length before the draft), every row read before any is written,

@@ -55,6 +55,7 @@ EXPORTED_SYMBOLS = (
     "xllm_hip_mrope_kv_write",
     "xllm_hip_tree_attention_workspace_bytes",
     "xllm_hip_tree_attention",
+    "xllm_hip_tree_attention_describe",
     "xllm_hip_move_accepted_tokens",
     "xllm_hip_set_option",
     "xllm_hip_get_option",
@@ -257,6 +258,8 @@ def load():
     lib.xllm_hip_tree_attention_workspace_bytes.restype = ctypes.c_size_t
     lib.xllm_hip_tree_attention.argtypes = [P(KvCacheDesc), P(DecodeArgs), vp, i64, i32, vp, ctypes.c_size_t, vp]
     lib.xllm_hip_tree_attention.restype = ctypes.c_int
+    lib.xllm_hip_tree_attention_describe.argtypes = [P(KvCacheDesc), P(DecodeArgs), P(ctypes.c_int64), i32]
+    lib.xllm_hip_tree_attention_describe.restype = ctypes.c_int
     lib.xllm_hip_move_accepted_tokens.argtypes = [P(KvCacheDesc), vp, i64, i32, vp, vp, i64, i32, vp, i32, vp, vp]
     lib.xllm_hip_move_accepted_tokens.restype = ctypes.c_int
     lib.xllm_hip_set_option.argtypes = [i32, i64]

@@ -263,26 +263,37 @@ static void launch_tree_mfma(int kv_dt, int rows_per_item, const TreeParams& p, 
   }
 }
 
-}  // namespace xllm_hip
-
-using namespace xllm_hip;
-
-extern "C" size_t xllm_hip_tree_attention_workspace_bytes(int32_t batch, int32_t q_per_seq, int32_t num_q_heads,
-                                                          int32_t num_kv_heads, int32_t head_dim) {
-  if (batch < 1 || q_per_seq < 1 || num_q_heads < 1 || num_kv_heads < 1 || head_dim < 1) return 0;
-  const int64_t s = tree_slots(batch, q_per_seq, num_q_heads, num_kv_heads, head_dim);
-  if (s == 1) return 0;
-  return tree_line_bytes(batch) + tree_lse_bytes(batch, q_per_seq, num_q_heads, s) + (size_t)(batch * s * q_per_seq * num_q_heads * head_dim * 4);
+// How a call is run: the form, and in `p` the sizes, how its sequences are cut and the items of the launch that follow.
+static TreeForm lay_out_tree(const xllm_hip_kv_cache* c, const xllm_hip_decode_args* a, TreeParams& p) {
+  p.batch = a->batch;
+  p.n = a->q_per_seq;
+  p.num_q_heads = a->num_q_heads;
+  p.num_kv_heads = c->num_kv_heads;
+  p.group = a->num_q_heads / c->num_kv_heads;
+  p.head_dim = c->head_dim;
+  p.slots = (int32_t)tree_slots(a->batch, p.n, p.num_q_heads, p.num_kv_heads, p.head_dim);
+  const TreeForm form = tree_form(c, a);
+  p.tile = form.rows_per_item > 0 ? 32 : 64;  // (what the kernels take at a time)
+  const int64_t rows = (int64_t)p.n * p.group;
+  p.row_groups = (int32_t)(form.rows_per_item > 0 ? (rows + form.rows_per_item - 1) / form.rows_per_item : rows);
+  p.rows_per_item = form.rows_per_item;
+  choose_chunks(a, form, elem_bytes(c->dtype), p);
+  return form;
 }
 
-extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
-                                       const xllm_hip_decode_args* a,
-                                       const uint64_t* tree_mask,
-                                       int64_t mask_stride,
-                                       int32_t mask_words,
-                                       void* workspace,
-                                       size_t workspace_bytes,
-                                       xllm_hip_stream_t stream) {
+// Workgroups of the attention launch.
+static int64_t tree_workgroups(const TreeForm& form, const TreeParams& p) {
+  int64_t items = (int64_t)p.batch * p.slots * p.num_kv_heads * p.row_groups;
+  if (p.pieces > 0) {
+    items = (int64_t)p.pieces * p.num_kv_heads;
+  } else if (form.rows_per_item > 0 && p.row_groups > 1) {  // whole rounds of the XCDs (see the kernel)
+    items = (items + kTreeXcds * p.row_groups - 1) / (kTreeXcds * p.row_groups) * (kTreeXcds * p.row_groups);
+  }
+  return items;
+}
+
+// What can be said of a call without its query, output, mask and workspace.
+static int check_tree_sizes(const xllm_hip_kv_cache* c, const xllm_hip_decode_args* a) {
   XLLM_HIP_REQUIRE(c != nullptr && a != nullptr, "cache or args is NULL");
   XLLM_HIP_REQUIRE(c->k_cache != nullptr && c->v_cache != nullptr, "k_cache or v_cache is NULL");
   XLLM_HIP_REQUIRE(c->num_blocks > 0 && c->num_blocks <= 0x7fffffff && c->block_size > 0 && c->num_kv_heads > 0 && c->head_dim > 0,
@@ -305,14 +316,13 @@ extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
   if (a->q_per_seq > kTreeMaxNodes) {
     return fail(XLLM_HIP_UNSUPPORTED, "q_per_seq %d is larger than %d", a->q_per_seq, kTreeMaxNodes);
   }
-  XLLM_HIP_REQUIRE(mask_words >= 1 && mask_stride >= mask_words, "mask rows need at least one word");
-  if (mask_words > kTreeMaxWords) {
-    return fail(XLLM_HIP_UNSUPPORTED, "mask_words %d is larger than %d", mask_words, kTreeMaxWords);
-  }
   if (a->batch > 65535) return fail(XLLM_HIP_UNSUPPORTED, "batch %d is larger than 65535", a->batch);
   XLLM_HIP_REQUIRE(a->max_seq_len >= 0 && a->total_kv_len >= 0, "max_seq_len or total_kv_len is negative");
-  if (a->batch == 0) return XLLM_HIP_OK;
-  XLLM_HIP_REQUIRE(a->q != nullptr && a->out != nullptr && tree_mask != nullptr, "q, out or tree_mask is NULL");
+  return XLLM_HIP_OK;
+}
+
+// The lists and strides of a call with sequences.
+static int check_tree_lists(const xllm_hip_kv_cache* c, const xllm_hip_decode_args* a) {
   if (a->block_table != nullptr) {
     XLLM_HIP_REQUIRE(a->seq_lens != nullptr, "block_table form needs seq_lens");
     XLLM_HIP_REQUIRE(a->max_blocks_per_seq >= 1 && a->block_table_stride >= a->max_blocks_per_seq, "bad block_table shape");
@@ -323,6 +333,39 @@ extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
   const int64_t rowlen = (int64_t)a->num_q_heads * c->head_dim;
   XLLM_HIP_REQUIRE(a->q_token_stride >= rowlen && a->out_token_stride >= rowlen,
                    "q/out token stride smaller than num_q_heads*head_dim");
+  return XLLM_HIP_OK;
+}
+
+}  // namespace xllm_hip
+
+using namespace xllm_hip;
+
+extern "C" size_t xllm_hip_tree_attention_workspace_bytes(int32_t batch, int32_t q_per_seq, int32_t num_q_heads,
+                                                          int32_t num_kv_heads, int32_t head_dim) {
+  if (batch < 1 || q_per_seq < 1 || num_q_heads < 1 || num_kv_heads < 1 || head_dim < 1) return 0;
+  const int64_t s = tree_slots(batch, q_per_seq, num_q_heads, num_kv_heads, head_dim);
+  if (s == 1) return 0;
+  return tree_line_bytes(batch) + tree_lse_bytes(batch, q_per_seq, num_q_heads, s) + (size_t)(batch * s * q_per_seq * num_q_heads * head_dim * 4);
+}
+
+extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
+                                       const xllm_hip_decode_args* a,
+                                       const uint64_t* tree_mask,
+                                       int64_t mask_stride,
+                                       int32_t mask_words,
+                                       void* workspace,
+                                       size_t workspace_bytes,
+                                       xllm_hip_stream_t stream) {
+  int rc = check_tree_sizes(c, a);
+  if (rc != XLLM_HIP_OK) return rc;
+  XLLM_HIP_REQUIRE(mask_words >= 1 && mask_stride >= mask_words, "mask rows need at least one word");
+  if (mask_words > kTreeMaxWords) {
+    return fail(XLLM_HIP_UNSUPPORTED, "mask_words %d is larger than %d", mask_words, kTreeMaxWords);
+  }
+  if (a->batch == 0) return XLLM_HIP_OK;
+  XLLM_HIP_REQUIRE(a->q != nullptr && a->out != nullptr && tree_mask != nullptr, "q, out or tree_mask is NULL");
+  rc = check_tree_lists(c, a);
+  if (rc != XLLM_HIP_OK) return rc;
   const size_t need = xllm_hip_tree_attention_workspace_bytes(a->batch, a->q_per_seq, a->num_q_heads, c->num_kv_heads, c->head_dim);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) {
     return fail(XLLM_HIP_WORKSPACE_TOO_SMALL, "workspace has %zu bytes, need %zu", workspace_bytes, need);
@@ -330,6 +373,8 @@ extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
   XLLM_HIP_REQUIRE(need == 0 || ((uintptr_t)workspace & 255) == 0, "workspace must be 256-byte aligned");
 
   TreeParams p{};
+  const int64_t slots = tree_slots(a->batch, a->q_per_seq, a->num_q_heads, c->num_kv_heads, c->head_dim);  // the workspace's
+  const TreeForm form = lay_out_tree(c, a, p);
   p.q = a->q;
   p.out = a->out;
   p.lse = a->lse;
@@ -359,36 +404,17 @@ extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
   p.sc_stride_block = c->scale_stride_block;
   p.sc_stride_head = c->scale_stride_head;
   p.sc_stride_slot = c->scale_stride_slot;
-  p.batch = a->batch;
-  p.n = a->q_per_seq;
-  p.num_q_heads = a->num_q_heads;
-  p.num_kv_heads = c->num_kv_heads;
-  p.group = a->num_q_heads / c->num_kv_heads;
-  p.head_dim = c->head_dim;
   p.block_size = c->block_size;
   p.log2_bs = is_pow2(c->block_size) ? ilog2(c->block_size) : -1;
   p.last_block = (int32_t)(c->num_blocks - 1);
   p.q_dtype = a->q_dtype;
   p.scale_log2 = (float)((double)a->sm_scale * 1.4426950408889634);
-  const int64_t slots = tree_slots(a->batch, p.n, p.num_q_heads, p.num_kv_heads, p.head_dim);
-  p.slots = (int32_t)slots;
   if (slots > 1) {
     p.line = (int64_t*)workspace;
     p.partial_lse = (float*)((uint8_t*)workspace + tree_line_bytes(a->batch));
     p.partial_out = (float*)((uint8_t*)p.partial_lse + tree_lse_bytes(a->batch, p.n, p.num_q_heads, slots));
   }
-  const TreeForm form = tree_form(c, a);
-  p.tile = form.rows_per_item > 0 ? 32 : 64;  // (what the kernels take at a time)
-  const int64_t rows = (int64_t)p.n * p.group;
-  p.row_groups = (int32_t)(form.rows_per_item > 0 ? (rows + form.rows_per_item - 1) / form.rows_per_item : rows);
-  p.rows_per_item = form.rows_per_item;
-  choose_chunks(a, form, elem_bytes(c->dtype), p);
-  int64_t items = (int64_t)p.batch * p.slots * p.num_kv_heads * p.row_groups;
-  if (p.pieces > 0) {
-    items = (int64_t)p.pieces * p.num_kv_heads;
-  } else if (form.rows_per_item > 0 && p.row_groups > 1) {  // whole rounds of the XCDs (see the kernel)
-    items = (items + kTreeXcds * p.row_groups - 1) / (kTreeXcds * p.row_groups) * (kTreeXcds * p.row_groups);
-  }
+  const int64_t items = tree_workgroups(form, p);
   XLLM_HIP_REQUIRE(items <= 0x7fffffff, "too many work items: %lld", (long long)items);
   hipStream_t st = (hipStream_t)stream;
   const unsigned grid = (unsigned)items;
@@ -405,7 +431,7 @@ extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
   } else {
     launch_tree_generic<XLLM_HIP_FP32>(c->dtype, p, grid, st);
   }
-  int rc = check_launch("tree attention kernel");
+  rc = check_launch("tree attention kernel");
   if (rc != XLLM_HIP_OK || (p.slots == 1 && p.pieces == 0)) return rc;
   if (p.q_dtype == XLLM_HIP_BF16) {
     launch_tree_merge<XLLM_HIP_BF16>(p, st);
@@ -415,4 +441,25 @@ extern "C" int xllm_hip_tree_attention(const xllm_hip_kv_cache* c,
     launch_tree_merge<XLLM_HIP_FP32>(p, st);
   }
   return check_launch("tree_merge_kernel");
+}
+
+extern "C" int xllm_hip_tree_attention_describe(const xllm_hip_kv_cache* c, const xllm_hip_decode_args* a, int64_t* out, int32_t count) {
+  XLLM_HIP_REQUIRE(out != nullptr && count >= 0, "out is NULL or count negative");
+  int rc = check_tree_sizes(c, a);
+  if (rc != XLLM_HIP_OK) return rc;
+  int64_t values[6] = {};
+  if (a->batch > 0) {
+    rc = check_tree_lists(c, a);
+    if (rc != XLLM_HIP_OK) return rc;
+    TreeParams p{};
+    const TreeForm form = lay_out_tree(c, a, p);
+    values[0] = form.rows_per_item;
+    values[1] = tree_workgroups(form, p);
+    values[2] = p.row_groups;
+    values[3] = p.pieces;
+    values[4] = p.pieces > 0 ? 0 : p.chunk;
+    values[5] = p.slots;
+  }
+  for (int i = 0; i < count; ++i) out[i] = i < 6 ? values[i] : 0;
+  return XLLM_HIP_OK;
 }

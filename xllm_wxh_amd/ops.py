@@ -714,6 +714,23 @@ def batch_tree_decode(query, k_cache, v_cache, output, block_table, seq_lens, tr
                               _nhd(kv_layout), max_seq_len, total_kv_len, workspace, indptr, indices, last_page_len)
 
 
+TREE_DESCRIBE_FIELDS = ("rows_per_workgroup", "workgroups", "row_groups", "line_pieces", "chunk_tokens", "chunk_slots")
+
+
+def tree_decode_describe(query, k_cache, v_cache, block_table, seq_lens, *, scale=1.0, q_indptr=None, q_per_seq=None,
+                         k_cache_quant_scale=None, v_cache_quant_scale=None, kv_layout="HND", max_seq_len=0, total_kv_len=0,
+                         csr=None):
+    """How batch_tree_decode would run these tensors (xllm_hip_tree_attention_describe: decided on the host, nothing is
+    launched): a dict of TREE_DESCRIBE_FIELDS."""
+    _require(q_per_seq is not None, "q_per_seq (the most query tokens of a sequence) is required")
+    desc = _cache_desc(k_cache, v_cache, k_cache_quant_scale, v_cache_quant_scale, kv_layout)
+    args, _keep = _decode_args(query, query, None, block_table, seq_lens, csr, q_per_seq, scale, -1, max_seq_len, desc, total_kv_len,
+                               q_indptr)
+    vals = (ctypes.c_int64 * len(TREE_DESCRIBE_FIELDS))()
+    _lib.check(_lib.load().xllm_hip_tree_attention_describe(ctypes.byref(desc), ctypes.byref(args), vals, len(TREE_DESCRIBE_FIELDS)))
+    return dict(zip(TREE_DESCRIBE_FIELDS, (int(v) for v in vals)))
+
+
 def move_accepted_tokens(k_cache, v_cache, block_table, cached_lens, accepted, num_accepted, new_lens=None, *,
                          k_cache_scale=None, v_cache_scale=None, kv_layout="HND"):
     """The cache rows of the accepted path moved to the front of the drafted range, for one layer's cache
