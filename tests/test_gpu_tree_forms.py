@@ -53,3 +53,22 @@ def test_chunks_without_hints(gpu, kv, n, Hkv, rows):
     f = form_of(c)
     assert f["line_pieces"] == 0 and f["rows_per_workgroup"] == rows and f["chunk_tokens"] == 256 and f["chunk_slots"] > 5, f
     c.check(*c.run())
+
+
+@pytest.mark.parametrize("stride,rows", [(71582789, 0), (2 ** 26 - 1, 32)])
+@pytest.mark.parametrize("kv", ["int8", "fp8"])
+def test_scales_far_apart(gpu, kv, stride, rows):
+    """Slot-major scale tensors of a very large cache: the scales of a block's 16 tokens lie up to 4.3 GB apart, past 32
+    bits of bytes, or just within."""
+    print("case far scales", kv, stride, flush=True)
+    c = TreeCase([6, 3], [90, 41], 8, 2, 128, 16, kv=kv, seed=34)
+    nb = c.ks.size(0)
+    far = []
+    for t in (c.ks, c.vs):
+        store = torch.empty(15 * stride + nb * 2, dtype=torch.float32, device=gpu)
+        view = store.as_strided((nb, 2, 16), (2, 1, stride))
+        view.copy_(t)
+        far.append(view)
+    c.ks, c.vs = far
+    assert form_of(c)["rows_per_workgroup"] == rows
+    c.check(*c.run())

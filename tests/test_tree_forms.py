@@ -57,6 +57,18 @@ def test_what_the_matrix_kernels_do_not_serve(lib, change):
     assert f["rows_per_workgroup"] == 0 and f["line_pieces"] == 0
 
 
+@pytest.mark.parametrize("bs", [16, 64])
+def test_scales_far_apart(lib, bs):
+    """The matrix kernels hold a token's scale as a 32-bit byte offset within its group of 16 tokens: 15 strides of
+    2^32 / 60 floats are the first that do not fit.  (From 2^30 / block_size floats on the generic kernel serves the call.)"""
+    for kv in (_lib.INT8, _lib.FP8_E4M3):
+        for stride in (71582789, 2 ** 31 // bs - 1, 2 ** 30 // bs):
+            assert describe(lib, 4, 8, 8, 2, 128, bs, kv=kv, scale_stride_slot=stride)["rows_per_workgroup"] == 0, stride
+        assert describe(lib, 4, 8, 8, 2, 128, bs, kv=kv, scale_stride_slot=2 ** 30 // bs - 1)["rows_per_workgroup"] == 32
+    # (strides of a 16-bit cache's scales, if any are given, are nobody's)
+    assert describe(lib, 4, 8, 8, 2, 128, bs, scale_stride_slot=2 ** 40)["rows_per_workgroup"] == 32
+
+
 def test_without_hints(lib):
     # 16-bit caches: the line from 64 (sequence, kv head, row group)s on; 8-bit ones never
     assert describe(lib, 64, 8, 8, 1, 128, 16)["line_pieces"] == 512

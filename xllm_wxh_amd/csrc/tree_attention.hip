@@ -86,7 +86,8 @@ static TreeForm tree_form(const xllm_hip_kv_cache* c, const xllm_hip_decode_args
   const int64_t vec = 16 / eb, lim = (int64_t)1 << 31;
   if (c->stride_block % vec != 0 || c->stride_head % vec != 0 || c->stride_slot % vec != 0) return none;
   if (c->stride_block >= lim || c->stride_slot * c->block_size >= lim) return none;
-  if (quant && (c->scale_stride_block >= lim || c->scale_stride_slot * c->block_size >= lim)) return none;
+  // (a lane's scale lies within 32 bits of bytes from its block's first: TreeLoader::sc_off)
+  if (quant && (c->scale_stride_block >= lim || c->scale_stride_slot * c->block_size >= lim / 2)) return none;
   if ((((uintptr_t)c->k_cache | (uintptr_t)c->v_cache | (uintptr_t)a->q | (uintptr_t)a->out) & 15) != 0) return none;
   if (a->q_token_stride % 8 != 0 || a->out_token_stride % 8 != 0) return none;
   const int64_t rows = (int64_t)a->q_per_seq * (a->num_q_heads / c->num_kv_heads);
