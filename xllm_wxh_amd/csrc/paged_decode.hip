@@ -127,7 +127,7 @@ static Variant pick_variant(const xllm_hip_kv_cache* c, const xllm_hip_decode_ar
     if (eb == 1) {
       scales_ok = c->k_scale != nullptr && c->v_scale != nullptr && c->scale_stride_block >= 0 &&
                   c->scale_stride_block < lim32 && c->scale_stride_slot >= 0 &&
-                  c->scale_stride_slot * c->block_size < lim32;
+                  c->scale_stride_slot * c->block_size < lim32 / 2;  // (a lane's scale: 32 bits of bytes)
     }
     const bool range_ok = c->stride_block >= 0 && c->stride_block < lim32 && c->stride_slot >= 0 &&
                           c->stride_slot * c->block_size < lim32;
