@@ -4,8 +4,10 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import paged_kv_oracle as orc
 from xllm_wxh_amd import ops
 
+from helpers import TORCH_KV_DTYPE, TORCH_Q_DTYPE
 from test_gpu_tree_attention import TreeCase
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +74,93 @@ def test_scales_far_apart(gpu, kv, stride, rows):
     c.ks, c.vs = far
     assert form_of(c)["rows_per_workgroup"] == rows
     c.check(*c.run())
+
+
+def far_below(kv, q, D, at, gap, n, L, layout="HND", seed=40):
+    """One key (token `at`) whose score is `gap` nats above the others' for every row, and whose value row is zero: the
+    output is made of weights far below the largest.  An 8-bit cache has one V scale for all tokens, so that its zero row
+    is no smaller than the others by its scale."""
+    c = TreeCase([n], [L], 8, 2, D, 16, q=q, kv=kv, layout=layout, seed=seed)
+    g = torch.Generator().manual_seed(seed)
+    qt = (1.0 + 0.25 * torch.randn(n, 8, D, generator=g)).to(TORCH_Q_DTYPE[q])
+    c.q_ref, c.q = qt.float().numpy(), qt.to(c.q.device)
+    nb = c.k_ref.shape[0]
+    kf, vf = 0.2 * torch.randn(nb, 2, 16, D, generator=g), torch.randn(nb, 2, 16, D, generator=g).abs() * 2.0 ** 12
+    blk, slot = int(c.table[0, at // 16]), at % 16
+    kf[blk, :, slot], vf[blk, :, slot] = gap / D ** 0.5, 0.0
+    if kv in ("int8", "fp8"):
+        qk, sk = orc.quantize_per_token_head(kf.numpy(), kv)
+        one = float(vf.abs().max()) / (127.0 if kv == "int8" else 448.0)
+        sv = torch.full((nb, 2, 16), one)
+        qv = (vf / one).round().to(torch.int8) if kv == "int8" else (vf / one).to(torch.float8_e4m3fn)
+        c.k_ref, c.v_ref = orc.dequantize(qk, sk, kv), (qv.float() * one).numpy()
+        tensors = [torch.from_numpy(qk.view(np.uint8)).view(TORCH_KV_DTYPE[kv]), qv, torch.from_numpy(sk), sv]
+    else:
+        tensors = [kf.to(TORCH_KV_DTYPE[kv]), vf.to(TORCH_KV_DTYPE[kv]), None, None]
+        c.k_ref, c.v_ref = tensors[0].float().numpy(), tensors[1].float().numpy()
+    c.k, c.v, c.ks, c.vs = (None if t is None else (t.swapaxes(1, 2).contiguous() if layout == "NHD" else t).to(c.q.device) for t in tensors)
+    return c
+
+
+def lost_below(c, D):
+    """What fp16's smallest number may cost an element of the output.  A weight is within 2^-11 of its value or within
+    2^-25.  Over a fp16 cache the largest weight of 32 tokens that are taken together is at least 2^-13, and that of the row's
+    largest token at least 2^10; over an 8-bit cache the row's largest is at least 2^4."""
+    L, n = int(c.lens[0]), c.counts[0]
+    k, v = (r[0].astype(np.float64) for r in (c.rows(c.k_ref), c.rows(c.v_ref)))
+    out = np.zeros((n, 8, D))
+    if c.kv == "bf16":  # (bf16 weights have a float's range)
+        return out
+    for j in range(n):
+        sees = np.array([t < L - n or (int(c.mask[j, 0]) >> (t - L + n)) & 1 for t in range(L)], bool)
+        for h in range(8):
+            x = k[:, h // 4] @ c.q_ref[j, h].astype(np.float64) * c.scale
+            p = np.where(sees, np.exp(x - x[sees].max()), 0.0)
+            p /= p.sum()
+            if c.kv == "fp16":
+                tops = np.repeat([p[i:i + 32].max() for i in range(0, L, 32)], 32)[:L]
+                tops *= np.where(tops == p.max(), 2.0 ** -35, 2.0 ** -12)
+            else:
+                tops = np.full(L, p.max() * 2.0 ** -29)
+            out[j, h] = (tops * sees) @ np.abs(v[:, h // 4])
+    return out
+
+
+@pytest.mark.parametrize("kv,q", [("fp16", "fp16"), ("int8", "bf16"), ("fp8", "fp16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("D,n,place", [(128, 4, 5), (128, 12, 1040), (64, 40, -1), (256, 20, 2066)])
+@pytest.mark.parametrize("gap", [10.0, 18.0])
+def test_weights_far_below_a_dominant_one(gpu, kv, q, D, n, place, gap):
+    """18 nats are 26 bits: such weights were 0 in fp16, and the output with them.  `place` -1: the first drafted token, which
+    is masked for some rows."""
+    print("case far below", kv, q, D, n, place, gap, flush=True)
+    L = 2100
+    c = far_below(kv, q, D, L - n if place < 0 else place, gap, n, L)
+    want = c.oracle()
+    two_u = torch.finfo(TORCH_Q_DTYPE[q]).eps
+    ref = (want[0], want[1], want[2] + lost_below(c, D) / two_u, want[3], want[4])
+    for hints in (dict(), dict(max_seq_len=L, total_kv_len=L), dict(max_seq_len=10 ** 6, total_kv_len=10 ** 6)):
+        c.check(*c.run(**hints), ref=ref)
+
+
+@pytest.mark.parametrize("gap", [10.0, 20.0])
+def test_weights_far_below_on_the_line(gpu, gap):
+    """The same over a fp16 cache on the line: the reference point of a row moves, and differs at the joins."""
+    c = far_below("fp16", "fp16", 128, 700, gap, 9, 2100, layout="NHD")
+    indptr = torch.tensor([0, 9] + [9] * 99, dtype=torch.int32, device=gpu)
+    table = torch.cat([c.d_table, c.d_table.new_zeros(99, c.d_table.size(1))])[:100].contiguous()
+    lens = torch.cat([c.d_lens, c.d_lens.new_full((99,), 40)])
+    kw = dict(q_indptr=indptr, table=table, lens=lens)
+    f = ops.tree_decode_describe(c.q, c.k, c.v, table, lens, scale=c.scale, q_indptr=indptr, q_per_seq=9, kv_layout="NHD")
+    assert f["line_pieces"] > 0
+    want = c.oracle()
+    ref = (want[0], want[1], want[2] + lost_below(c, 128) / 2.0 ** -10, want[3], want[4])
+    c.check(*c.run(**kw), ref=ref)
+
+
+def test_scores_that_scatter_widely(gpu):
+    """Scores that scatter by ten nats: over a fp16 cache the reference points move up and down all the time."""
+    for n in (6, 40):
+        c = TreeCase([n, n], [3000, 1777], 8, 2, 128, 16, q="fp16", kv="fp16", seed=41, std=10.0)
+        want = c.oracle()
+        c.check(*c.run(), ref=want)
+        c.check(*c.run(max_seq_len=3000, total_kv_len=4777), ref=want)

@@ -13,7 +13,8 @@
 //         0 it is the subnormal (x + 128) 2^-24, and the row takes back 128 times the sum of its query's elements with
 //         the factor that its scores get anyway.  (Twice 128 is the most that this adds to a product, so the fp32 sums
 //         lose about a bit.  V has no such end: there the 128 would pile up over the tokens.)
-// With V in fp16 the weights of an 8-bit cache are rounded to 11 bits, those over a bf16 cache to 8.
+// With V in fp16 the weights of an fp16 or 8-bit cache are rounded to 11 bits, those over a bf16 cache to 8; how fp16's range
+// is kept from cutting into them stands at TreeRows::kFollow.
 //
 // How the waves share an item: 128 rows to a workgroup are 32 to each wave, which then reads all of the tile, and 64 rows
 // over a 16-bit cache 16.  Up to 32 rows are two tiles of 16: over a 16-bit cache two waves share a row tile, taking
@@ -36,6 +37,8 @@
 
 #include "decode_mfma.h"
 #include "tree_params.h"
+
+#include <float.h>
 
 namespace xllm_hip {
 
@@ -357,11 +360,26 @@ struct TreeRows {
       q_bias = -128.0f * kg_sum(sum) * q_scale;
       q_scale *= 0x1p24f;
     }
-    m_run = -INFINITY;
+    m_run = SH::kQuant ? -FLT_MAX : -INFINITY;
     l_run = 0.0f;
 #pragma unroll
     for (int dt = 0; dt < SH::kDT; ++dt) acc[dt] = f32x4{0, 0, 0, 0};
   }
+
+  // Where the largest weight of a piece may lie (log 2).  Where V is fp16 so are the weights, and one far enough below the
+  // reference point would be rounded to few bits, or to 0, while its share stays in the sum: a key that dominates a row but
+  // has a tiny V would hide what the others add.
+  //   fp16 cache    the reference point follows the pieces, down too (kFollow): a piece's largest weight stays within
+  //                 2^kLow .. 2^kTop, so what fp16's end at 2^-25 costs is at most 2^-12 of that weight; of the row's
+  //                 largest, which is at least 2^(kTop - 5), 2^-35.  (64 x 8192 tokens, 128 rows: 409 us before and after;
+  //                 430 where scores scatter by 6 nats and the point moves often)
+  //   8-bit cache   a weight holds its token's V scale, so it says what the token can add; the largest is between 2^kHead
+  //                 and 2^(kHead + kLazyRescale), a smaller one costs 2^-29 of it at most.  (Following the pieces took 4 to 6 %
+  //                 from the forms that vector instructions bound.)
+  //   bf16 cache    bf16 weights have a float's range.
+  static constexpr bool kFollow = SH::kVF16 && !SH::kQuant;
+  static constexpr float kTop = 15.0f, kLow = -13.0f, kMost = 60.0f;
+  static constexpr float kHead = SH::kQuant ? 4.0f : 0.0f;
 
   // The scale rides in the FMA that forms the exponent where nothing else needs the scaled score.
   template <bool MASKED>
@@ -394,13 +412,35 @@ struct TreeRows {
     for (int i = 0; i < 8; ++i) mt = fmaxf(mt, x[i]);
     mt = kg_max(mt);
     if (kFold<MASKED>) mt *= scale_log2;
-    // The reference point of the exponents follows the running maximum lazily: it moves when a row's maximum has grown
-    // by more than kLazyRescale (in log 2).  Weights up to that are harmless, and the accumulators are seldom rescaled.
-    const float m_top = fmaxf(m_run, mt);
-    const bool moved = __builtin_amdgcn_ballot_w64(m_top > m_run + kLazyRescale) != 0;
-    const float m_new = moved ? m_top : m_run;
-    const float m_safe = m_new == neg_inf ? 0.0f : m_new;
-    alpha = __builtin_amdgcn_exp2f(m_run - m_safe);
+    // The reference point of the exponents follows the scores lazily, so that the accumulators are seldom rescaled.  (It
+    // begins at -FLT_MAX over an 8-bit cache, where a guard against -inf - -inf would cost two instructions a piece.)
+    float m_new, m_safe;
+    bool moved;
+    if constexpr (kFollow) {
+      const float d = mt - m_run;
+      moved = __builtin_amdgcn_ballot_w64(!(fabsf(d - (kTop + kLow) * 0.5f) <= (kTop - kLow) * 0.5f)) != 0;
+      m_new = m_run;
+      if (moved) {
+        // (not so far down that what has been summed up could pass 2^kMost; of a row that has seen a token l_run is above 1)
+        const float low = m_run + (__builtin_amdgcn_logf(kg_max(l_run)) - kMost);
+        if (d > kTop) m_new = mt - kTop + 5.0f;
+        if (d < kLow && mt > neg_inf) m_new = fmaxf(mt - kLow - 5.0f, fminf(m_run, low));
+      }
+      m_safe = m_new == neg_inf ? 0.0f : m_new;
+      alpha = __builtin_amdgcn_exp2f(m_run - m_safe);
+    } else {
+      // It moves when a row's maximum has grown by more than kLazyRescale (in log 2).
+      const float m_top = fmaxf(m_run, mt);
+      moved = __builtin_amdgcn_ballot_w64(m_top > m_run + kLazyRescale) != 0;
+      m_new = moved ? m_top : m_run;
+      if constexpr (SH::kQuant) {
+        m_safe = m_new - kHead;
+        alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      } else {
+        m_safe = m_new == neg_inf ? 0.0f : m_new;
+        alpha = __builtin_amdgcn_exp2f(m_run - m_safe);
+      }
+    }
     l_run *= alpha;
     m_run = m_new;
 #pragma unroll
@@ -607,7 +647,7 @@ __device__ __forceinline__ void tree_mfma_item(const TreeParams& p, const TreeIt
     f32x4 rvs[2];
     factor(stage, piece, 2, rvs);
     const uint32_t vo = fresh(v_off);
-    constexpr int kFetched = SH::kNormQ && TS == 1 ? SH::kDT - 1 : SH::kDT;  // (all of them would spill)
+    constexpr int kFetched = TS == 1 ? SH::kDT - 1 : SH::kDT;  // (all of them would spill)
     i32x2 vraw[kAhead ? SH::kDT : 1];
     if constexpr (kAhead) {
 #pragma unroll
@@ -802,7 +842,7 @@ __device__ __forceinline__ void tree_mfma_item(const TreeParams& p, const TreeIt
         l += w[x] * ml[x * kApart * RTW * 32 + 16];
       }
       TreeOut out;
-      if (!out.init(p, it, first_row + 16 * a, end_lane, l, m, tg == 0 && end_kg == 0)) continue;
+      if (!out.init(p, it, first_row + 16 * a, end_lane, l, m - Rows::kHead, tg == 0 && end_kg == 0)) continue;
 #pragma unroll
       for (int q = 0; q < SH::kDT / TS; ++q) {
         const int dt = tg * (SH::kDT / TS) + q;
@@ -823,7 +863,7 @@ __device__ __forceinline__ void tree_mfma_item(const TreeParams& p, const TreeIt
     Rows& r = rows[a];
     const float l = kg_sum(r.l_run);
     TreeOut out;
-    if (!out.init(p, it, first_row + 16 * a, end_lane, l, r.m_run, end_kg == 0)) continue;
+    if (!out.init(p, it, first_row + 16 * a, end_lane, l, r.m_run - Rows::kHead, end_kg == 0)) continue;
 #pragma unroll
     for (int dt = 0; dt < SH::kDT; ++dt) out.template store<SH::kQF16>(dt * 16 + 4 * end_kg, r.acc[dt]);
   }
