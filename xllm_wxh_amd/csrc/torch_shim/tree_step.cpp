@@ -5,11 +5,9 @@
 #include <hip/hip_runtime_api.h>
 
 #include <limits>
-#include <map>
-#include <mutex>
-#include <utility>
 
 #include "../../../include/xllm_hip_paged_kv.h"
+#include "stream_scratch.h"
 
 namespace xllm::kernel::hip {
 namespace {
@@ -129,17 +127,15 @@ void mask_words(const torch::Tensor& t, int64_t rows) {
 
 // One buffer per (device, stream) for eager calls, grown to the largest call's need: the buffer that is outgrown goes
 // back to torch's allocator, which hands it out again in the order of the stream.
-torch::Tensor tree_workspace(const c10::Device& dev, xllm_hip_stream_t stream, size_t bytes) {
-  const auto options = torch::TensorOptions().dtype(torch::kUInt8).device(dev);
-  hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
-  (void)hipStreamIsCapturing((hipStream_t)stream, &capturing);
-  if (capturing != hipStreamCaptureStatusNone) return torch::empty({(int64_t)bytes}, options);
-  static std::mutex mutex;
-  static auto* buffers = new std::map<std::pair<int, void*>, torch::Tensor>();  // (outlives the allocator's teardown)
-  std::lock_guard<std::mutex> lock(mutex);
-  torch::Tensor& ws = (*buffers)[{(int)dev.index(), stream}];
-  if (!ws.defined() || (size_t)ws.numel() < bytes) ws = torch::empty({(int64_t)bytes}, options);
-  return ws;
+StreamScratch<torch::Tensor>& tree_scratch() {
+  static auto* scratch = new StreamScratch<torch::Tensor>();  // (outlives the allocator's teardown)
+  return *scratch;
+}
+
+bool is_capturing(xllm_hip_stream_t stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  (void)hipStreamIsCapturing((hipStream_t)stream, &status);
+  return status != hipStreamCaptureStatusNone;
 }
 
 }  // namespace
@@ -379,18 +375,23 @@ void batch_tree_decode(const torch::Tensor& query, const torch::Tensor& k_cache,
   if (rows == 0) return;
   const c10::DeviceGuard guard(dev);
   const xllm_hip_stream_t stream = stream_of(dev);
-  torch::Tensor ws;
+  const auto attend = [&](const torch::Tensor& ws) {
+    check(xllm_hip_tree_attention(&cache, &a, (const uint64_t*)tree_mask.data_ptr(), row_stride(tree_mask),
+                                  as_i32(tree_mask.size(1), "mask words"), ws.defined() ? ws.data_ptr() : nullptr,
+                                  ws.defined() ? (size_t)ws.nbytes() : 0, stream));
+  };
   if (has(workspace)) {
     TREE_REQUIRE(workspace->is_contiguous(), "workspace must be contiguous");
-    ws = *workspace;
-  } else {
-    const size_t need =
-        xllm_hip_tree_attention_workspace_bytes(a.batch, a.q_per_seq, a.num_q_heads, cache.num_kv_heads, cache.head_dim);
-    if (need > 0) ws = tree_workspace(dev, stream, need);
+    return attend(*workspace);
   }
-  check(xllm_hip_tree_attention(&cache, &a, (const uint64_t*)tree_mask.data_ptr(), row_stride(tree_mask),
-                                as_i32(tree_mask.size(1), "mask words"), ws.defined() ? ws.data_ptr() : nullptr,
-                                ws.defined() ? (size_t)ws.nbytes() : 0, stream));
+  const size_t need = xllm_hip_tree_attention_workspace_bytes(a.batch, a.q_per_seq, a.num_q_heads, cache.num_kv_heads, cache.head_dim);
+  if (need == 0) return attend(torch::Tensor());
+  const auto options = torch::TensorOptions().dtype(torch::kUInt8).device(dev);
+  if (is_capturing(stream)) return attend(torch::empty({(int64_t)need}, options));
+  const auto held = tree_scratch().hold(dev.index(), stream);  // until both launches are enqueued
+  torch::Tensor& ws = *held;
+  if (!ws.defined() || (size_t)ws.numel() < need) ws = torch::empty({(int64_t)need}, options);
+  attend(ws);
 }
 
 void move_accepted_tokens(const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& block_table,

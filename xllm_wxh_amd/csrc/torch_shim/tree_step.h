@@ -76,8 +76,9 @@ void mrope_kv_write(const torch::Tensor& qkv,
                     bool nhd);
 
 // xllm_hip_tree_attention.  block_table and seq_lens, or the three csr arrays.  Without `workspace` the scratch is one
-// buffer per (device, stream), grown to the largest call's need; under stream capture it is memory of the graph's own
-// pool, so that no two graphs, and no graph and no eager call, share one.
+// buffer per (device, stream), grown to the largest call's need and held while the call's launches are enqueued, so that
+// several host threads may use one stream; under stream capture it is memory of the graph's own pool, so that no two
+// graphs, and no graph and no eager call, share one.  A `workspace` of the caller's serves one call at a time.
 void batch_tree_decode(const torch::Tensor& query,
                        const torch::Tensor& k_cache,
                        const torch::Tensor& v_cache,
