@@ -164,3 +164,64 @@ def test_scores_that_scatter_widely(gpu):
         want = c.oracle()
         c.check(*c.run(), ref=want)
         c.check(*c.run(max_seq_len=3000, total_kv_len=4777), ref=want)
+
+
+def poisoned(c, victims):
+    """Runs the case clean, then with NaN (and infinities) in the V and K rows of one drafted token per sequence and of
+    every slot behind the sequences: rows that do not see the token keep their result, those that do have none."""
+    clean, clean_lse = c.run()
+    blind = np.ones(c.q.size(0), bool)
+    places = []
+    for b, n in enumerate(c.counts):
+        L = int(c.lens[b])
+        end = -(-L // c.bs) * c.bs
+        places += [(int(c.table[b, t // c.bs]), t % c.bs) for t in range(L, end)]
+        if n > L or victims[b] is None:
+            continue
+        t, lo = L - n + victims[b], int(c.q_indptr[b])
+        places.append((int(c.table[b, t // c.bs]), t % c.bs))
+        for j in range(n):
+            blind[lo + j] = not (int(c.mask[lo + j, victims[b] // 64]) >> (victims[b] % 64)) & 1
+    assert blind.any() and not blind.all()
+    blind = torch.from_numpy(blind).to(c.q.device)
+    blk, slot = (torch.tensor(x, device=c.q.device) for x in zip(*places))
+    u = torch.finfo(c.q.dtype).eps
+    for what in (float("nan"),) if c.kv == "fp8" else (float("nan"), float("inf")):
+        bad = torch.full((1,), what, device=c.q.device).to(c.k.dtype).view(torch.uint8 if c.kv == "fp8" else torch.int16)
+        for cache in (c.v, c.k):
+            bits = cache.view(bad.dtype)
+            keep = bits.clone()
+            bits[blk, :, slot] = bad
+            got, lse = c.run()
+            assert torch.isfinite(got[blind].float()).all()
+            # (the piece is then summed token by token, with the weights' own bits: half a step of the weights and of the
+            # output, on either side; V is normal, so sums of its products stay below a few units)
+            assert torch.allclose(got[blind].float(), clean[blind].float(), rtol=2 * u, atol=2 * u)
+            assert torch.allclose(lse[blind], clean_lse[blind], rtol=1e-5, atol=1e-5)
+            if cache is c.v or what != what:
+                assert not torch.isfinite(got[~blind].float()).any()
+            bits.copy_(keep)
+
+
+@pytest.mark.parametrize("kv,q", [("bf16", "bf16"), ("fp16", "fp16"), ("fp8", "bf16")])
+@pytest.mark.parametrize("n,L,victims,Hq,D", [(6, 259, (1, 4), 8, 128), (12, 262, (3, 8), 8, 128), (40, 275, (5, 35), 8, 128), (20, 266, (2, 15), 4, 256),
+                                              (12, 520, (2, 9), 14, 64)])
+def test_unseen_places_on_both_sides_of_a_cut(gpu, kv, q, n, L, victims, Hq, D):
+    """The drafted range lies across the chunks' border at a multiple of 256 tokens; merged afterwards."""
+    print("case poison cut", kv, n, D, flush=True)
+    for victim in victims:
+        c = TreeCase([n], [L], Hq, 2, D, 16, q=q, kv=kv, seed=60 + n)
+        f = form_of(c)
+        assert f["line_pieces"] == 0 and f["chunk_tokens"] == 256 and f["chunk_slots"] > 1 and (L - n) // 256 < (L - 1) // 256
+        poisoned(c, [victim])
+
+
+@pytest.mark.parametrize("q", ["bf16", "fp16"])
+@pytest.mark.parametrize("Hq,D,most", [(8, 128, 8), (8, 128, 13), (16, 128, 20), (14, 64, 4), (8, 256, 20)])
+def test_unseen_places_on_the_line(gpu, q, Hq, D, most):
+    print("case poison line", q, Hq, D, most, flush=True)
+    counts, lens = ragged(34, most, 300, most + 1)
+    lens = np.maximum(lens, counts)
+    c = TreeCase(counts, lens, Hq, 2, D, 16, q=q, kv=q, seed=70 + most)
+    assert form_of(c)["line_pieces"] > 0
+    poisoned(c, [None if n < 2 else n // 2 for n in counts])
