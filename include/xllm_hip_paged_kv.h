@@ -557,6 +557,8 @@ int xllm_hip_gather_from_cache(const xllm_hip_kv_cache* cache,
  * free_head_out[0] = *free_head + blocks taken, free_head_out[1] = blocks that were needed and could not be had
  * (the free list, or W, was too short): such a block appears as 0 in the table, its tokens get slot -1.
  * Earlier sequences are served first, so the result depends on nothing but the inputs.
+ * q_indptr and kv_indptr are not cut to num_rows and kv_indices_capacity: what reads them needs num_rows >= the sum of n and
+ * kv_indices_capacity >= the sum of min(need, table_width) (batch * table_width is always enough).
  * Inputs and outputs must not overlap except block_pool; request_ids must differ from each other when blocks
  * are taken.  Lengths below 0 count as 0; a request id outside [0, pool_rows) holds no blocks and takes none;
  * a block id that is negative, or whose slot does not fit 32 bits, gives slot -1.  batch <= 4096.
@@ -653,7 +655,8 @@ int xllm_hip_mrope_kv_write(const xllm_hip_rope_args* args,
  * (bits past mask_words count as clear).  The mask need not be a tree's: any bits are served.  What a row does not
  * see takes no part in it whatever it holds (NaN and infinities included); a row that sees nothing yields zeros and
  * lse = -inf.  args as for xllm_hip_paged_decode: either block-list form, q_indptr or q_per_seq, every cache layout
- * and type, lse optional; max_seq_len and total_kv_len are hints that only tune how sequences are cut (0 = unknown).
+ * and type, lse optional; max_seq_len and total_kv_len are hints that only tune how sequences are cut (0 = unknown), and with
+ * it the order in which sums are formed.  Rows must not lie behind the query: q_indptr[batch] rows are read and written.
  * A sliding window (window_left >= 0) and host_plan are refused: XLLM_HIP_UNSUPPORTED.  mask_words <= 8; q_per_seq
  * <= 512 is the largest n_b; tokens past it are ignored.  batch <= 65535.  A quantised cache's V scales must not be
  * negative (no quantiser makes such), and one below 2^-100 may count as 2^-100 in the weights' sum of products.

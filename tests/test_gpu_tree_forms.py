@@ -225,3 +225,25 @@ def test_unseen_places_on_the_line(gpu, q, Hq, D, most):
     c = TreeCase(counts, lens, Hq, 2, D, 16, q=q, kv=q, seed=70 + most)
     assert form_of(c)["line_pieces"] > 0
     poisoned(c, [None if n < 2 else n // 2 for n in counts])
+
+
+@pytest.mark.parametrize("kv", ["int8", "fp8"])
+@pytest.mark.parametrize("every", [1, 2])
+def test_scales_of_zero(gpu, kv, every):
+    """Tokens whose scales are zero (a cache that was never written): their score is 0 and they add nothing, but they keep
+    their share of the weights' sum.  `every` 1: all tokens are so, and the output is zero, up to this: a V scale below 2^-100 may
+    count as 2^-100, and |V| is at most 448 before its scale, so an element may be off by 448 * 2^-100 = 3.5e-28."""
+    little = 448 * 2.0 ** -100
+    for n, L in ((6, 6000), (20, 700), (40, 6000)):
+        print("case scales of zero", kv, every, n, flush=True)
+        c = TreeCase([n], [L], 8, 2, 128, 16, kv=kv, seed=36)
+        for t in (c.ks, c.vs):
+            t[:, :, ::every] = 0.0
+        c.k_ref[:, :, ::every], c.v_ref[:, :, ::every] = 0.0, 0.0
+        want = c.oracle()
+        ref = (want[0], want[1], want[2] + little / 2.0 ** -7, want[3], want[4])  # (2^-7: twice half a step of bf16)
+        for hints in (dict(), dict(max_seq_len=L, total_kv_len=L)):
+            out, lse = c.run(**hints)
+            c.check(out, lse, ref=ref)
+            if every == 1:
+                assert float(out.float().abs().max()) <= little

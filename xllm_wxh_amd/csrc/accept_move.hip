@@ -8,9 +8,9 @@
 // touches those bytes.
 //
 // Little memory traffic behind a chain of three dependent loads (length, path and table entry, row), so what counts is
-// how many chains run side by side: one launch for K, V and the scales, as few pieces to a thread as keep the grid near
-// two thousand workgroups (more only queue), and few registers (512 sequences, paths of 13 rows of fp8: 27 us with eight
-// pieces to every thread and the scales in a launch of their own, 9 so).
+// how many chains run side by side: one launch for K, V and the scales, as few pieces to a thread as keep K and V near
+// two thousand workgroups (more only queue; the scales' have little to do), and few registers (512 sequences, paths of
+// 13 rows of fp8: 27 us with eight pieces to every thread and the scales in a launch of their own, 9 so).
 #include "device_utils.h"
 #include "host_utils.h"
 
@@ -192,7 +192,8 @@ extern "C" int xllm_hip_move_accepted_tokens(const xllm_hip_kv_cache* cache,
     XLLM_HIP_REQUIRE(cols <= 0x7fffffff, "too many kv heads");
     p.cols[a] = (int32_t)cols;
   }
-  // Pieces to a thread: as few as make a grid of at most 2048 workgroups; a workgroup takes a path's whole columns.
+  // Pieces to a thread: as few as make at most 2048 workgroups for K and V, kMovePieces at most; a workgroup takes a path's
+  // whole columns.
   const int arrays = quant ? 4 : 2;
   const int path = path_width > 0 ? path_width : 1;
   int pieces = 1;

@@ -11,8 +11,8 @@
 // into LDS, for all of the token's heads (each head fetching it by itself asks the caches for the row 40 times and
 // picks the axis 40 times).  Then D / 8 lanes to a head, eight elements (16 bytes of a 16-bit type) to a lane; a
 // rotation partner is a shuffle away.  The bound is memory: q and k heads read and written, v heads read, K and V
-// rows written (8191 bf16 tokens of 32 + 8 + 8 heads of 128, norm, 16-bit cache: 51 us for 223 MB, 4.4 TB/s where a
-// large copy runs at 5.0; 136 drafted tokens of 14 + 2 + 2 heads of 64: 4.1 us, a launch).  Other head sizes, strides
+// rows written (8191 bf16 tokens of 32 + 8 + 8 heads of 128, norm, 16-bit cache: 51 us for 223 MB, 4.3 TB/s where a
+// large copy runs at 5.0; 136 drafted tokens of 14 + 2 + 2 heads of 64: 4.6 us, a launch).  Other head sizes, strides
 // and rotary dims take a wave per head, an element to a lane.
 #include "device_utils.h"
 #include "host_utils.h"

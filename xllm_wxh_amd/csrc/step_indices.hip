@@ -6,7 +6,7 @@
 // Both are launch-bound: the arrays of a decode step are kilobytes, those of a large mixed step a megabyte.  So
 // each is one launch in which no workgroup waits for another: a workgroup that needs sums over the sequences in
 // front of its own forms them itself from the lengths (4096 sequences at most: 48 KiB, from L2).  8 sequences of 4096
-// tokens, one new token each: 4.8 us; 255 sequences of up to 9001 tokens and 700 new ones: 7.8, the loads of the
+// tokens, one new token each: 5.0 us; 255 sequences of up to 9001 tokens and 700 new ones: 7.3, the loads of the
 // lengths, the scan, the search for a row's sequence and the load of its block one after another.
 #include "device_utils.h"
 #include "host_utils.h"
@@ -172,8 +172,8 @@ __device__ inline void table_part(const StepParams& p, int wg, int64_t* lds) {
 }
 
 // What the token rows need of the sequences: exclusive sums of token counts and of blocks taken; up to 512 sequences
-// also what seq_need fetched, so that a row does not wait for it again (255 sequences 8.7 -> 7.8 us; the 96 KiB of 4096
-// sequences would leave a CU one workgroup: 2000 sequences 16.9 -> 22.5).
+// also what seq_need fetched, so that a row does not wait for it again (255 sequences: a tenth less time; the 96 KiB of 4096
+// sequences would leave a CU one workgroup: 2000 sequences 16.9 -> 22.5 us).
 template <int N>
 struct StepSums {
   static constexpr bool kKept = N <= 512;
@@ -300,8 +300,8 @@ __global__ void __launch_bounds__(kStepThreads) step_indices_kernel(StepParams p
 // doubles the stretch of ancestors A(v) covers, so ceil(log2 (depth + 1)) steps finish any tree (a chain of 512 nodes
 // takes nine; a walk up it would take 511 dependent reads; a random tree of 300 nodes takes four).  One workgroup per
 // sequence, one thread per node, the words of all nodes in LDS; the depth is the number of bits set, less the node
-// itself.  Bound by the launch and three dependent loads (192 trees of up to 300 nodes: 5.4 us; 6.0 with eight
-// words and nine steps for all of them).
+// itself.  Bound by the launch, two dependent loads (offsets, parents), the doubling's barriers and the load of the base
+// behind them (192 trees of up to 300 nodes: 5.4 us; 6.0 with eight words and nine steps for all of them).
 // ---------------------------------------------------------------------------------
 struct TreeMaskParams {
   const int32_t* parents;

@@ -7,7 +7,7 @@
 // Long sequences are cut into chunks of whole tiles, a workgroup each; a chunk leaves a normalised partial and its
 // base-2 log-sum-exp, and tree_merge_kernel joins them.  How a sequence is cut follows from its own length, read on
 // the device, and two numbers from the host (tokens per chunk, chunks a sequence may have), so any hints, stale ones
-// of a captured graph included, give the same result.
+// of a captured graph included, give the same result up to the rounding of sums that are formed in another order.
 #include "device_utils.h"
 #include "host_utils.h"
 #include "tree_generic.h"
@@ -99,12 +99,15 @@ static TreeForm tree_form(const xllm_hip_kv_cache* c, const xllm_hip_decode_args
 }
 
 // Tokens per chunk and chunks per sequence (at most p.slots of them on entry), or pieces of a line.  Without the host's
-// lengths: from 64 (sequence, kv head, row group)s on the line where it serves (64 x 4096 bf16 tokens, 8 drafts: 170 us
-// against 208 in chunks; 2 x 700 tokens, 16 of them, 16 against 12), else chunks of at least
-// kTreeMinChunk tokens, as many to a sequence as make 1024 items (with 2048, 32 x 8192 fp8 tokens and 512 query rows to a
-// kv head take 848 us against 673).  With them, the cut whose step is predicted to end first, from what a token costs
-// where all workgroups run (`slots` of them): its K and V at the memory's rate, or its products at that of the matrix
-// kernels, whichever is more,
+// lengths: from 64 (sequence, kv head, row group)s on the line where it serves, else chunks of at least kTreeMinChunk tokens, as
+// many to a sequence as make 1024 items (with 2048, 32 x 8192 fp8 tokens and 512 query rows to a kv head take 848 us against
+// 673).  Where the two meet, bf16, 8 kv heads of 128, 8 drafts, ragged, us in chunks / on the line:
+//   up to 1000 tokens   32 items 13.8 / 17.3   64 items 14.8 / 18.5   128 items 18.6 / 22.2   256 items  31.7 /  29.7
+//             4000               17.5 / 22.0            29.0 / 26.3             45.2 / 42.3              76.6 /  70.1
+//            16000               46.2 / 41.8            76.0 / 70.0            138.2 / 122.8
+// (head_dim 256 and 128 query rows gain more from it: 64 items of 4000 tokens 61.1 / 45.0 and 45.2 / 38.1.)
+// With them, the cut whose step is predicted to end first, from what a token costs where all workgroups run (`slots` of
+// them): its K and V at the memory's rate, or its products at that of the matrix kernels, whichever is more,
 //   nearly equal lengths   rounds of equal items:  ceil(items / slots) * (chunk + start)
 //   ragged lengths         the longest chunk while all items run together; else the items' tokens over `slots`, and
 //                          half a chunk until the last one ends
@@ -140,7 +143,7 @@ static void choose_chunks(const xllm_hip_decode_args* a, const TreeForm& form, i
   const bool equal = longest * p.batch * 4 <= total * 5;
   const double lanes = (double)p.num_kv_heads * p.row_groups;
   const double rows = (double)p.n * p.group < form.rows_per_item ? (double)p.n * p.group : (double)form.rows_per_item;
-  // ns (6.5 bytes, 850 kflop in one)
+  // ns (6.5 kB or 850 kflop in one)
   const double bytes = 2.0 * p.head_dim * eb * form.slots / 6.5e3;
   const double flops = 4.0 * p.head_dim * form.rows_per_item * form.slots / 850e3;
   const double token = bytes > flops ? bytes : flops;

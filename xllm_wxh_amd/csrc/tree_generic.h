@@ -12,7 +12,7 @@ namespace xllm_hip {
 // over the chunk with the running maximum m and sum l of the softmax,
 //   m' = max(m, max_t x_t),  l' = l 2^(m - m') + sum_t 2^(x_t - m'),  o' = o 2^(m - m') + sum_t 2^(x_t - m') v_t,
 // in floats; a token the row does not see is given x = -inf and its V is never read.  Not tuned (one dependent
-// cache row per lane): it serves the shapes the matrix kernels do not, and checks them.
+// cache row per lane): it serves the shapes the matrix kernels do not.
 template <int Q_DT, int KV_DT>
 __global__ void __launch_bounds__(64) tree_generic_kernel(TreeParams p) {
   __shared__ __attribute__((aligned(16))) float qs[256];

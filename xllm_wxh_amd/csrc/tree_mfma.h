@@ -13,8 +13,9 @@
 //         0 it is the subnormal (x + 128) 2^-24, and the row takes back 128 times the sum of its query's elements with
 //         the factor that its scores get anyway.  (Twice 128 is the most that this adds to a product, so the fp32 sums
 //         lose about a bit.  V has no such end: there the 128 would pile up over the tokens.)
-// With V in fp16 the weights of an fp16 or 8-bit cache are rounded to 11 bits, those over a bf16 cache to 8; how fp16's range
-// is kept from cutting into them stands at TreeRows::kFollow.
+// Both operands of a matrix instruction have one type.  So with V in fp16 the weights of an fp16 or 8-bit cache are rounded to
+// 11 bits — how fp16's range is kept from cutting into them stands at TreeRows::kFollow — and those over a bf16 cache to 8: a
+// bf16 V has no exact fp16 form, and two bf16 numbers to a weight would double the second product.
 //
 // How the waves share an item: 128 rows to a workgroup are 32 to each wave, which then reads all of the tile, and 64 rows
 // over a 16-bit cache 16.  Up to 32 rows are two tiles of 16: over a 16-bit cache two waves share a row tile, taking
@@ -24,8 +25,8 @@
 // (16 rows or fewer): a step this narrow is bound by memory.
 //
 // Measured, kernel and merge, bf16 queries, head_dim 128, block_size 16 unless stated:
-//   16-bit cache, 8 or 16 drafts of 4 heads to a kv head, 64 x 4096 or 8192 tokens   164 / 331 us   6.5 TB/s: memory
-//   512 rows to a kv head, 32 x 8192 tokens   bf16 648 us, 850 TFLOP/s; fp8 662 us, 830; int8 770 us, 715: the softmax's
+//   16-bit cache, 8 or 16 drafts of 4 heads to a kv head, 64 x 4096 or 8192 tokens   165 / 335 us   6.5 TB/s: memory
+//   512 rows to a kv head, 32 x 8192 tokens   bf16 652 us, 843 TFLOP/s; fp8 661 us, 831; int8 760 us, 723: the softmax's
 //   and the widening's vector instructions, which the matrix instructions of one wave only partly cover for another
 //
 // Only the last tokens of a sequence are drafted ones, so only the last pieces are masked.  There a row takes from its
